@@ -93,7 +93,8 @@ typedef struct mhlik_config {
 int mhlik_create(const mhlik_config *config, mhlik_ctx **out);
 void mhlik_destroy(mhlik_ctx *ctx);
 
-/* Last error text of this context (ctx == NULL: of the last failed create). */
+/* Last error text of this context (ctx == NULL: of the last failed create, or of the last failed call that takes no
+ * context, on this thread). */
 const char *mhlik_last_error(const mhlik_ctx *ctx);
 
 /* Global row range [begin, begin+count) this shard holds. */
@@ -427,6 +428,86 @@ int mhlik_autocorrelation_f64(mhlik_ctx *ctx, const double *samples, int64_t n, 
                               double *out_v, double *sum);
 int mhlik_autocorrelation_f32(mhlik_ctx *ctx, const float *samples, int64_t n, int32_t d, int32_t lags,
                               float *out_v, float *sum);
+
+/* ---- answers from posterior draws ----------------------------------------
+ *
+ * What a chain's kept draws are used for: the predictor x_i.theta_s of new rows
+ * under thousands of draws (mhlik_q8_product; the K-chain passes above take
+ * at most MHLIK_MAX_BATCH and reduce over the rows), and a draw of one column
+ * of a row of log weights from a given random number (mhlik_draw).  No
+ * counterpart in the reference, which writes its samples to a file
+ * (src/util/io.c) and stops.
+ *
+ * These calls take no context.  All arrays are DEVICE memory of one GPU,
+ * `device` is its ordinal (-1: the current one; the caller's current device
+ * is restored), `stream` a stream of that GPU (a hipStream_t; NULL: its default
+ * stream).  A call queues its kernels there and returns: it allocates
+ * nothing, waits for nothing and can be captured into a graph.  Different
+ * threads and streams may call at the same time; a workspace serves one call
+ * at a time (captured ones included).  Errors: mhlik_last_error(NULL). */
+enum { MHLIK_T_Q8 = 0, MHLIK_T_F64 = 1, MHLIK_T_F32 = 2, MHLIK_T_BF16 = 3, MHLIK_T_F16 = 4 }; /* element types */
+
+/* Rows in 8 bits (MHLIK_T_Q8).  A row of `cols` values is cut into blocks of 128 columns; block b of row i holds
+ *   data [i][128 b + c] = e4m3(x 2^-k)   (to nearest even, from the exact quotient)
+ *   scale[i][b]         = k + 127,       k the least integer in [-96, 119] with |x| <= 448 2^k for the block's finite x
+ * data has 128 ceil(cols/128) bytes a row (columns past the last: 0), starts at a multiple of 16 bytes; scale has
+ * 4 ceil(cols/512) bytes a row (spare ones: 127).  Values that are not finite, or exceed 448 2^119, become NaN.
+ * x[i * row_stride + c * col_stride], of any type but MHLIK_T_Q8; strides count elements and are not negative.
+ * 0 <= rows <= 2^40, 1 <= cols <= 2^22. */
+int mhlik_q8_quantize(const void *x, int32_t type, int64_t rows, int64_t cols, int64_t row_stride, int64_t col_stride,
+                      uint8_t *data, uint8_t *scale, int32_t device, void *stream);
+
+/* out[i * out_stride + s] = sum_c x[i][c] w[s][c] over the values that the 8-bit rows stand for.  x may be 8-bit rows
+ * (x_type MHLIK_T_Q8: x and x_scale) or values, which are quantized first, into the workspace.  out is float (products
+ * and sums as exact as float sums are), bfloat16 or half (products as the 8-bit matrix instructions add them: 1.6e-5 of
+ * the result's norm before the rounding).  The padding of 8-bit rows must be zeros, and out must not overlap the inputs. */
+typedef struct mhlik_q8_operands {
+  const void *x;          /* [rows] */
+  const uint8_t *x_scale; /* MHLIK_T_Q8 only */
+  int64_t x_row_stride;   /* values only */
+  int64_t x_col_stride;
+  const uint8_t *w_data;  /* [draws] */
+  const uint8_t *w_scale;
+  void *out;
+  int64_t out_stride;     /* >= draws */
+  int64_t rows, draws, cols;
+  void *workspace;        /* values only: mhlik_q8_product_workspace(rows, cols) bytes at a multiple of 16 */
+  size_t workspace_bytes;
+  int32_t x_type;
+  int32_t out_type;
+} mhlik_q8_operands;
+int mhlik_q8_product_workspace(int64_t rows, int64_t cols, size_t *bytes);
+int mhlik_q8_product(const mhlik_q8_operands *operands, int32_t device, void *stream);
+
+/* One column of each row of log weights z[i * stride + j], j < n (float, bfloat16 or half), by a random number u[i] in
+ * [0, 1) (double or float):
+ *   w_j = exp((z_j - max) / temperature);  z_j = -inf: 0
+ *   in the order of z, largest first, equal ones by column, keep
+ *     the first top_k                                              (top_k <= 0 or >= n: all)
+ *     those before which less than top_p of the mass of these lies (top_p >= 1: all; the first always)
+ *     those with w_j >= min(min_p, 1)                              (min_p <= 0: all)
+ *   index[i] = the first column, in column order, at which the kept mass exceeds u of the whole of it
+ *   logp[i]  = log(w_index / kept mass)                            (logp may be NULL)
+ * Sums are taken in double.  temperature 0: the largest, the lowest column of equal ones.  A row without a weight above
+ * -inf, with a NaN, or whose u, temperature, top_p or min_p is NaN (or the temperature negative): index -1, logp NaN.
+ * u outside [0, 1) counts as its nearest end.  temperature .. min_p: device arrays of one value a row, or NULL and the
+ * *_all value for every row.  0 <= rows < 2^31, 1 <= n < 2^30. */
+typedef struct mhlik_draw_rows {
+  const void *z;
+  int64_t rows, n, stride;
+  const void *u;
+  const float *temperature;
+  const int32_t *top_k;
+  const float *top_p;
+  const float *min_p;
+  double temperature_all, top_p_all, min_p_all;
+  int64_t *index;
+  float *logp;
+  int32_t top_k_all;
+  int32_t z_type, u_type;
+  int32_t reserved;
+} mhlik_draw_rows;
+int mhlik_draw(const mhlik_draw_rows *rows, int32_t device, void *stream);
 
 /* ---- multi-GPU (no counterpart: the reference is single-GPU, mcmc_gpu.cu:28) */
 

@@ -100,6 +100,22 @@ class KChainBatch(C.Structure):
                 ("kernel_samples", C.c_int32)]
 
 
+class Q8Operands(C.Structure):
+    _fields_ = [("x", C.c_void_p), ("x_scale", C.c_void_p), ("x_row_stride", C.c_int64), ("x_col_stride", C.c_int64),
+                ("w_data", C.c_void_p), ("w_scale", C.c_void_p), ("out", C.c_void_p), ("out_stride", C.c_int64),
+                ("rows", C.c_int64), ("draws", C.c_int64), ("cols", C.c_int64), ("workspace", C.c_void_p),
+                ("workspace_bytes", C.c_size_t), ("x_type", C.c_int32), ("out_type", C.c_int32)]
+
+
+class DrawRows(C.Structure):
+    _fields_ = [("z", C.c_void_p), ("rows", C.c_int64), ("n", C.c_int64), ("stride", C.c_int64), ("u", C.c_void_p),
+                ("temperature", C.c_void_p), ("top_k", C.c_void_p), ("top_p", C.c_void_p), ("min_p", C.c_void_p),
+                ("temperature_all", C.c_double), ("top_p_all", C.c_double), ("min_p_all", C.c_double),
+                ("index", C.c_void_p), ("logp", C.c_void_p), ("top_k_all", C.c_int32), ("z_type", C.c_int32),
+                ("u_type", C.c_int32), ("reserved", C.c_int32)]
+
+
+T_Q8, T_F64, T_F32, T_BF16, T_F16 = 0, 1, 2, 3, 4
 KCHAIN_F64, KCHAIN_F32, KCHAIN_MP = 1, 2, 3
 
 
@@ -164,6 +180,10 @@ _SIGS = [
     ("mhlik_kchain_state", C.c_int, [_P, _P, _P]),
     ("mhlik_autocorrelation_f64", C.c_int, [_P, _P, C.c_int64, C.c_int32, C.c_int32, _P, C.POINTER(C.c_double)]),
     ("mhlik_autocorrelation_f32", C.c_int, [_P, _P, C.c_int64, C.c_int32, C.c_int32, _P, C.POINTER(C.c_float)]),
+    ("mhlik_q8_quantize", C.c_int, [_P, C.c_int32, C.c_int64, C.c_int64, C.c_int64, C.c_int64, _P, _P, C.c_int32, _P]),
+    ("mhlik_q8_product_workspace", C.c_int, [C.c_int64, C.c_int64, C.POINTER(C.c_size_t)]),
+    ("mhlik_q8_product", C.c_int, [C.POINTER(Q8Operands), C.c_int32, _P]),
+    ("mhlik_draw", C.c_int, [C.POINTER(DrawRows), C.c_int32, _P]),
     ("mhlik_comm_make_id", C.c_int, [_P]),
     ("mhlik_comm_init", C.c_int, [_P, _P]),
     ("mhlik_comm_destroy", C.c_int, [_P]),

@@ -26,6 +26,7 @@
 #include "mhlik_kchain.hpp"
 #include "mhlik_stats.hpp"
 #include "mhlik_synth.h"
+#include "mhlik_internal.h"
 
 using namespace mhlik;
 
@@ -272,6 +273,21 @@ int fail(mhlik_ctx *c, int code, const char *fmt, ...)
     g_create_error = buf;
   return code;
 }
+
+} // namespace
+
+int mhlik::fail_no_ctx(int code, const char *fmt, ...)
+{
+  char buf[512];
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(buf, sizeof buf, fmt, ap);
+  va_end(ap);
+  g_create_error = buf;
+  return code;
+}
+
+namespace {
 
 #define HIPCHK(c, expr)                                                                              \
   do {                                                                                               \

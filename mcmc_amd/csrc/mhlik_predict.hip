@@ -1,0 +1,273 @@
+// mhlik_predict.hip -- C-ABI of the predictive operators (include/mhlik.h, "answers from posterior draws"): checks,
+// variant choice and launches of mhlik_q8.hpp and mhlik_draw.hpp.  All data are on the device and stay there; a call
+// queues its kernels on the caller's stream, allocates nothing and waits for nothing.
+#include "mhlik.h"
+
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+
+#include "mhlik_draw.hpp"
+#include "mhlik_internal.h"
+#include "mhlik_q8.hpp"
+
+using namespace mhlik;
+
+namespace {
+
+#define PCHK(expr)                                                                                             \
+  do {                                                                                                         \
+    hipError_t e_ = (expr);                                                                                    \
+    if (e_ != hipSuccess)                                                                                      \
+      return fail_no_ctx(e_ == hipErrorOutOfMemory ? MHLIK_ENOMEM : MHLIK_EHIP, "%s failed: %s (%s:%d)", #expr, \
+                         hipGetErrorString(e_), __FILE__, __LINE__);                                           \
+  } while (0)
+
+// The device a call names is current until the call returns; the caller's comes back.
+class OnDevice {
+public:
+  explicit OnDevice(int device)
+  {
+    err = hipGetDevice(&before);
+    if (err == hipSuccess && device >= 0 && device != before) {
+      err = hipSetDevice(device);
+      changed = err == hipSuccess;
+    }
+  }
+  ~OnDevice()
+  {
+    if (changed) (void)hipSetDevice(before);
+  }
+  hipError_t err;
+
+private:
+  int before = 0;
+  bool changed = false;
+};
+
+size_t type_size(int32_t type)
+{
+  return type == MHLIK_T_F64 ? 8 : type == MHLIK_T_F32 ? 4 : type == MHLIK_T_BF16 || type == MHLIK_T_F16 ? 2 : 0;
+}
+
+bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
+
+// 128 rows of a matrix are reached with 31-bit offsets
+constexpr int64_t kMaxCols = (int64_t)1 << 22;
+constexpr int64_t kMaxRows = (int64_t)1 << 40;
+
+int check_rows8(const char *what, const void *data, const void *scale, int64_t rows)
+{
+  if (rows && (!data || !scale)) return fail_no_ctx(MHLIK_EINVAL, "%s: data and scale must not be NULL", what);
+  if (!aligned16(data)) return fail_no_ctx(MHLIK_EINVAL, "%s: data must start at a multiple of 16 bytes", what);
+  return MHLIK_OK;
+}
+
+template <typename T>
+int quantize_launch(const T *x, int64_t rows, int64_t cols, int64_t rs, int64_t cs, uint8_t *data, uint8_t *scale, hipStream_t stream)
+{
+  const int64_t blocks = q8_blocks(cols), sstride = q8_scale_stride(cols);
+  // Column by column if columns are contiguous and there are rows enough for a wave's loads to be (a wave of the row
+  // kernel would touch 64 lines for 64 values); a single row is both: the row kernel spreads it over more lanes.
+  if (rs == 1 && cs != 1 && rows >= 16) {
+    const int64_t groups = (rows + kBlock - 1) / kBlock;
+    if (groups > INT32_MAX || blocks > 65535) return fail_no_ctx(MHLIK_EINVAL, "too many rows or columns (%lld x %lld)", (long long)rows, (long long)cols);
+    hipLaunchKernelGGL(q8_columns_kernel<T>, dim3((unsigned)groups, (unsigned)blocks), dim3(kBlock), 0, stream, x, rows, cols, cs,
+                       (uint32_t)blocks, (uint32_t)sstride, data, scale);
+  } else {
+    const int64_t units = rows * blocks, groups = (units * 16 + kBlock - 1) / kBlock;
+    if (groups > INT32_MAX) return fail_no_ctx(MHLIK_EINVAL, "too many blocks (%lld)", (long long)units);
+    const bool vec = cs == 1 && aligned16(x) && (rows == 1 || rs * (int64_t)sizeof(T) % 16 == 0);
+    if (vec)
+      hipLaunchKernelGGL((q8_rows_kernel<T, true>), dim3((unsigned)groups), dim3(kBlock), 0, stream, x, units, cols, rs, cs,
+                         (uint32_t)blocks, (uint32_t)sstride, data, scale);
+    else
+      hipLaunchKernelGGL((q8_rows_kernel<T, false>), dim3((unsigned)groups), dim3(kBlock), 0, stream, x, units, cols, rs, cs,
+                         (uint32_t)blocks, (uint32_t)sstride, data, scale);
+  }
+  PCHK(hipGetLastError());
+  return MHLIK_OK;
+}
+
+int quantize(const void *x, int32_t type, int64_t rows, int64_t cols, int64_t rs, int64_t cs, uint8_t *data, uint8_t *scale,
+             hipStream_t stream)
+{
+  switch (type) {
+  case MHLIK_T_F64: return quantize_launch((const double *)x, rows, cols, rs, cs, data, scale, stream);
+  case MHLIK_T_F32: return quantize_launch((const float *)x, rows, cols, rs, cs, data, scale, stream);
+  case MHLIK_T_BF16: return quantize_launch((const __bf16 *)x, rows, cols, rs, cs, data, scale, stream);
+  default: return quantize_launch((const _Float16 *)x, rows, cols, rs, cs, data, scale, stream);
+  }
+}
+
+int check_shape(int64_t rows, int64_t cols)
+{
+  if (rows < 0 || rows > kMaxRows || cols < 1 || cols > kMaxCols)
+    return fail_no_ctx(MHLIK_EINVAL, "need 0 <= rows <= 2^40 and 1 <= cols <= 2^22 (rows=%lld cols=%lld)", (long long)rows, (long long)cols);
+  return MHLIK_OK;
+}
+
+int check_values(const char *what, const void *x, int32_t type, int64_t rows, int64_t rs, int64_t cs)
+{
+  if (!type_size(type)) return fail_no_ctx(MHLIK_EINVAL, "%s: unknown element type %d", what, type);
+  if (rows && !x) return fail_no_ctx(MHLIK_EINVAL, "%s must not be NULL", what);
+  if ((uintptr_t)x % type_size(type)) return fail_no_ctx(MHLIK_EINVAL, "%s: not aligned to its type", what);
+  if (rs < 0 || cs < 0) return fail_no_ctx(MHLIK_EINVAL, "%s: strides must not be negative (%lld, %lld)", what, (long long)rs, (long long)cs);
+  return MHLIK_OK;
+}
+
+template <typename T> int product_launch(Q8Product a, hipStream_t stream)
+{
+  a.aligned = (uintptr_t)a.out % (4 * sizeof(T)) == 0 && a.os % 4 == 0;
+  // Up to 64 rows a wave keeps all of them beside 16 draws, so that the draws are read once for all rows; more rows go
+  // to the tiles, which read the draws once per 128 rows.
+  if (a.rows <= 64) {
+    const int rf = a.rows <= 16 ? 1 : a.rows <= 32 ? 2 : 4;
+    const int64_t groups16 = (a.draws + 15) / 16;
+    int ks = 1; // waves that share 16 draws: until the chip's 1024 SIMDs have two each, or a wave's part is two steps
+    while (ks < 16 && groups16 * ks < 2048 && a.blocks >= 4 * ks) ks *= 2;
+    const int waves = ks < 4 ? 4 : ks;
+    const int64_t groups = (groups16 + waves / ks - 1) / (waves / ks);
+    if (groups > INT32_MAX) return fail_no_ctx(MHLIK_EINVAL, "too many draws (%lld)", (long long)a.draws);
+    const dim3 grid((unsigned)groups), block(waves * kWave);
+    if (rf == 1)
+      hipLaunchKernelGGL((q8_skinny_kernel<T, 1>), grid, block, 0, stream, a, ks);
+    else if (rf == 2)
+      hipLaunchKernelGGL((q8_skinny_kernel<T, 2>), grid, block, 0, stream, a, ks);
+    else
+      hipLaunchKernelGGL((q8_skinny_kernel<T, 4>), grid, block, 0, stream, a, ks);
+  } else {
+    const int64_t tm = (a.rows + kQ8Tile - 1) / kQ8Tile, tn = (a.draws + kQ8Tile - 1) / kQ8Tile;
+    if (tm * tn > INT32_MAX) return fail_no_ctx(MHLIK_EINVAL, "too large a product (%lld x %lld)", (long long)a.rows, (long long)a.draws);
+    hipLaunchKernelGGL((q8_tile_kernel<T, sizeof(T) == 4>), dim3((unsigned)(tm * tn)), dim3(kBlock), 0, stream, a, (int)tn);
+  }
+  PCHK(hipGetLastError());
+  return MHLIK_OK;
+}
+
+template <typename T> int draw_launch(const DrawArgs &a, hipStream_t stream)
+{
+  int shift = 63;
+  while (((int64_t)1 << (63 - shift)) < a.n) shift--;
+  if (a.n <= 4096)
+    hipLaunchKernelGGL((draw_row_kernel<T, 256>), dim3((unsigned)a.rows), dim3(256), 0, stream, a, shift);
+  else
+    hipLaunchKernelGGL((draw_row_kernel<T, 1024>), dim3((unsigned)a.rows), dim3(1024), 0, stream, a, shift);
+  PCHK(hipGetLastError());
+  return MHLIK_OK;
+}
+
+} // namespace
+
+extern "C" {
+
+int mhlik_q8_quantize(const void *x, int32_t type, int64_t rows, int64_t cols, int64_t row_stride, int64_t col_stride, uint8_t *data,
+                      uint8_t *scale, int32_t device, void *stream)
+{
+  if (int rc = check_shape(rows, cols)) return rc;
+  if (int rc = check_values("x", x, type, rows, row_stride, col_stride)) return rc;
+  if (int rc = check_rows8("output", data, scale, rows)) return rc;
+  if (rows == 0) return MHLIK_OK;
+  OnDevice on(device);
+  PCHK(on.err);
+  return quantize(x, type, rows, cols, row_stride, col_stride, data, scale, (hipStream_t)stream);
+}
+
+int mhlik_q8_product_workspace(int64_t rows, int64_t cols, size_t *bytes)
+{
+  if (!bytes) return fail_no_ctx(MHLIK_EINVAL, "bytes must not be NULL");
+  if (int rc = check_shape(rows, cols)) return rc;
+  *bytes = (size_t)rows * (size_t)(q8_blocks(cols) * kQ8Block + q8_scale_stride(cols));
+  return MHLIK_OK;
+}
+
+int mhlik_q8_product(const mhlik_q8_operands *p, int32_t device, void *stream)
+{
+  if (!p) return fail_no_ctx(MHLIK_EINVAL, "operands must not be NULL");
+  if (int rc = check_shape(p->rows, p->cols)) return rc;
+  if (int rc = check_shape(p->draws, p->cols)) return rc;
+  if (int rc = check_rows8("w", p->w_data, p->w_scale, p->draws)) return rc;
+  const bool ready = p->x_type == MHLIK_T_Q8;
+  if (ready) {
+    if (int rc = check_rows8("x", p->x, p->x_scale, p->rows)) return rc;
+  } else {
+    if (int rc = check_values("x", p->x, p->x_type, p->rows, p->x_row_stride, p->x_col_stride)) return rc;
+  }
+  if (p->out_type != MHLIK_T_F32 && p->out_type != MHLIK_T_BF16 && p->out_type != MHLIK_T_F16)
+    return fail_no_ctx(MHLIK_EINVAL, "out: unknown element type %d", p->out_type);
+  if (p->rows == 0 || p->draws == 0) return MHLIK_OK;
+  if (!p->out || (uintptr_t)p->out % type_size(p->out_type)) return fail_no_ctx(MHLIK_EINVAL, "out is NULL or not aligned to its type");
+  if (p->out_stride < p->draws)
+    return fail_no_ctx(MHLIK_EINVAL, "out_stride=%lld is less than draws=%lld", (long long)p->out_stride, (long long)p->draws);
+  OnDevice on(device);
+  PCHK(on.err);
+  Q8Product a;
+  a.rows = p->rows;
+  a.draws = p->draws;
+  a.blocks = (int32_t)q8_blocks(p->cols);
+  a.kp = (int64_t)a.blocks * kQ8Block;
+  a.sstride = (int32_t)q8_scale_stride(p->cols);
+  a.w = p->w_data;
+  a.ws = p->w_scale;
+  a.out = p->out;
+  a.os = p->out_stride;
+  if (ready) {
+    a.x = (const uint8_t *)p->x;
+    a.xs = p->x_scale;
+  } else {
+    const size_t need = (size_t)p->rows * (size_t)(a.kp + a.sstride);
+    if (!p->workspace || !aligned16(p->workspace) || p->workspace_bytes < need)
+      return fail_no_ctx(MHLIK_EINVAL, "workspace: %zu bytes at a multiple of 16 are needed (%zu given)", need, p->workspace_bytes);
+    uint8_t *data = (uint8_t *)p->workspace, *scale = data + p->rows * a.kp;
+    if (int rc = quantize(p->x, p->x_type, p->rows, p->cols, p->x_row_stride, p->x_col_stride, data, scale, (hipStream_t)stream)) return rc;
+    a.x = data;
+    a.xs = scale;
+  }
+  switch (p->out_type) {
+  case MHLIK_T_F32: return product_launch<float>(a, (hipStream_t)stream);
+  case MHLIK_T_BF16: return product_launch<__bf16>(a, (hipStream_t)stream);
+  default: return product_launch<_Float16>(a, (hipStream_t)stream);
+  }
+}
+
+int mhlik_draw(const mhlik_draw_rows *p, int32_t device, void *stream)
+{
+  if (!p) return fail_no_ctx(MHLIK_EINVAL, "rows must not be NULL");
+  if (p->rows < 0 || p->rows > INT32_MAX || p->n < 1 || p->n >= INT32_MAX / 2)
+    return fail_no_ctx(MHLIK_EINVAL, "need 0 <= rows < 2^31 and 1 <= n < 2^30 (rows=%lld n=%lld)", (long long)p->rows, (long long)p->n);
+  if (p->z_type != MHLIK_T_F32 && p->z_type != MHLIK_T_BF16 && p->z_type != MHLIK_T_F16)
+    return fail_no_ctx(MHLIK_EINVAL, "z: unknown element type %d", p->z_type);
+  if (p->u_type != MHLIK_T_F64 && p->u_type != MHLIK_T_F32) return fail_no_ctx(MHLIK_EINVAL, "u: unknown element type %d", p->u_type);
+  if (int rc = check_values("z", p->z, p->z_type, p->rows, p->stride, 0)) return rc;
+  if (p->rows && (!p->u || !p->index)) return fail_no_ctx(MHLIK_EINVAL, "u and index must not be NULL");
+  if (!p->temperature && !(p->temperature_all == 0.0 || (p->temperature_all >= 1e-100 && p->temperature_all <= HUGE_VAL)))
+    return fail_no_ctx(MHLIK_EINVAL, "the temperature is 0 (the largest weight) or at least 1e-100 (%g)", p->temperature_all);
+  if (!p->top_p && p->top_p_all != p->top_p_all) return fail_no_ctx(MHLIK_EINVAL, "top_p is not a number");
+  if (!p->min_p && p->min_p_all != p->min_p_all) return fail_no_ctx(MHLIK_EINVAL, "min_p is not a number");
+  if (p->rows == 0) return MHLIK_OK;
+  OnDevice on(device);
+  PCHK(on.err);
+  DrawArgs a;
+  a.z = p->z;
+  a.rows = p->rows;
+  a.n = p->n;
+  a.stride = p->stride;
+  a.u = p->u;
+  a.u_is_double = p->u_type == MHLIK_T_F64;
+  a.temperature = p->temperature;
+  a.top_k = p->top_k;
+  a.top_p = p->top_p;
+  a.min_p = p->min_p;
+  a.temperature_all = p->temperature_all;
+  a.top_k_all = p->top_k_all;
+  a.top_p_all = p->top_p_all;
+  a.min_p_all = p->min_p_all;
+  a.index = p->index;
+  a.logp = p->logp;
+  switch (p->z_type) {
+  case MHLIK_T_F32: return draw_launch<float>(a, (hipStream_t)stream);
+  case MHLIK_T_BF16: return draw_launch<__bf16>(a, (hipStream_t)stream);
+  default: return draw_launch<_Float16>(a, (hipStream_t)stream);
+  }
+}
+}
