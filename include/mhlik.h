@@ -503,10 +503,13 @@ typedef struct mhlik_draw_rows {
   double temperature_all, top_p_all, min_p_all;
   int64_t *index;
   float *logp;
+  void *workspace;        /* mhlik_draw_workspace(rows, n) bytes at a multiple of 16 (may be 0) */
+  size_t workspace_bytes;
   int32_t top_k_all;
   int32_t z_type, u_type;
   int32_t reserved;
 } mhlik_draw_rows;
+int mhlik_draw_workspace(int64_t rows, int64_t n, size_t *bytes);
 int mhlik_draw(const mhlik_draw_rows *rows, int32_t device, void *stream);
 
 /* ---- multi-GPU (no counterpart: the reference is single-GPU, mcmc_gpu.cu:28) */

@@ -111,7 +111,8 @@ class DrawRows(C.Structure):
     _fields_ = [("z", C.c_void_p), ("rows", C.c_int64), ("n", C.c_int64), ("stride", C.c_int64), ("u", C.c_void_p),
                 ("temperature", C.c_void_p), ("top_k", C.c_void_p), ("top_p", C.c_void_p), ("min_p", C.c_void_p),
                 ("temperature_all", C.c_double), ("top_p_all", C.c_double), ("min_p_all", C.c_double),
-                ("index", C.c_void_p), ("logp", C.c_void_p), ("top_k_all", C.c_int32), ("z_type", C.c_int32),
+                ("index", C.c_void_p), ("logp", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+                ("top_k_all", C.c_int32), ("z_type", C.c_int32),
                 ("u_type", C.c_int32), ("reserved", C.c_int32)]
 
 
@@ -183,6 +184,7 @@ _SIGS = [
     ("mhlik_q8_quantize", C.c_int, [_P, C.c_int32, C.c_int64, C.c_int64, C.c_int64, C.c_int64, _P, _P, C.c_int32, _P]),
     ("mhlik_q8_product_workspace", C.c_int, [C.c_int64, C.c_int64, C.POINTER(C.c_size_t)]),
     ("mhlik_q8_product", C.c_int, [C.POINTER(Q8Operands), C.c_int32, _P]),
+    ("mhlik_draw_workspace", C.c_int, [C.c_int64, C.c_int64, C.POINTER(C.c_size_t)]),
     ("mhlik_draw", C.c_int, [C.POINTER(DrawRows), C.c_int32, _P]),
     ("mhlik_comm_make_id", C.c_int, [_P]),
     ("mhlik_comm_init", C.c_int, [_P, _P]),

@@ -56,6 +56,156 @@ __device__ __forceinline__ double draw_weight(float z, float max, double inv_t)
   return z == -HUGE_VALF ? 0.0 : mhlik_exp_fast(fmax(d * inv_t, -800.0));
 }
 
+
+// The choices of one row.
+struct DrawChoice {
+  double temp, inv_t, share, least, u; // least: at most 1
+  int k;                               // 0: no top-k
+  bool bad, greedy;                    // a choice that is not a number; temperature 0
+};
+
+__device__ inline DrawChoice draw_choice(const DrawArgs &a, int64_t row)
+{
+  DrawChoice c;
+  c.temp = a.temperature ? (double)a.temperature[row] : a.temperature_all;
+  c.share = a.top_p ? (double)a.top_p[row] : a.top_p_all;
+  c.least = a.min_p ? (double)a.min_p[row] : a.min_p_all;
+  c.u = a.u_is_double ? ((const double *)a.u)[row] : (double)((const float *)a.u)[row];
+  c.k = a.top_k ? a.top_k[row] : a.top_k_all;
+  if (c.k <= 0 || c.k >= a.n) c.k = 0;
+  c.bad = !(c.temp >= 0.0) || c.share != c.share || c.least != c.least || c.u != c.u;
+  c.greedy = c.temp == 0.0;
+  c.inv_t = c.greedy ? 1.0 : 1.0 / c.temp;
+  c.share = c.share > 0.0 ? c.share : 0.0;
+  if (c.least > 1.0) c.least = 1.0;
+  return c;
+}
+
+__device__ inline void draw_answer(const DrawArgs &a, int64_t row, int64_t column, double logp)
+{
+  a.index[row] = column;
+  if (a.logp) a.logp[row] = (float)logp;
+}
+
+__device__ inline void draw_nothing(const DrawArgs &a, int64_t row)
+{
+  a.index[row] = -1;
+  if (a.logp) a.logp[row] = __uint_as_float(0x7fc00000u);
+}
+
+// Values by distance from the largest: bin 0 holds the largest.  Distances beyond `range` share the last bin.
+template <int BINS> struct DrawBin {
+  float max, scale;
+  __device__ DrawBin(float max_, float min_, double temp) : max(max_)
+  {
+    // Weights e^-40 below the largest matter to no sum here, while a row may hold a lowest-of-its-type mask: the range
+    // is the nearer of the two.  All equal: one bin.
+    const float range = fminf((float)(40.0 * temp), max_ - min_);
+    scale = range > 0.f ? (float)BINS / range : 0.f;
+    if (!(scale < __uint_as_float(0x7f800000u))) scale = 0x1p127f; // a range below the smallest normal float
+  }
+  __device__ __forceinline__ int of(float z) const
+  {
+    return z == max ? 0 : (int)fminf((max - z) * scale, (float)(BINS - 1));
+  }
+};
+
+__device__ __forceinline__ unsigned long long draw_fixed(double w, int shift) { return (unsigned long long)rint(ldexp(w, shift)); }
+
+__device__ __forceinline__ double draw_wave_sum(double v)
+{
+#pragma unroll
+  for (int d = 1; d < kWave; d <<= 1) v += __shfl_xor(v, d);
+  return v;
+}
+
+// Position in the order: smaller is earlier (larger value, lower column).
+__device__ __forceinline__ unsigned long long draw_place(float z, int j)
+{
+  return (unsigned long long)~draw_key(z) << 32 | (uint32_t)j;
+}
+
+// The kept prefix ends with this place.
+struct DrawEnd {
+  unsigned long long place;
+  __device__ __forceinline__ bool kept(float z, int j) const { return draw_place(z, j) <= place; }
+};
+
+// The first column whose running sum exceeds `aim`, over weights w[i] at places base + i * 64 + lane of a wave's run;
+// base: the wave's first place, waves in order.  IS_SHARE: aim is a share of the whole sum, which comes back in *total.
+// On return place >= 0 in the one lane that has it, with its *weight and what is left of the aim where it begins (*rest).
+template <int THREADS, int VPT, bool IS_SHARE>
+__device__ int draw_pick(const double (&w)[VPT], double aim, double *total, double *weight, double *rest, double *lds /* [THREADS / 64] */)
+{
+  constexpr int kWaves = THREADS / kWave;
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  double m = 0.0;
+#pragma unroll
+  for (int i = 0; i < VPT; i++) m += w[i];
+  m = draw_wave_sum(m);
+  __syncthreads();
+  if (lane == 0) lds[wave] = m;
+  __syncthreads();
+  if (IS_SHARE) {
+    double t = 0.0;
+#pragma unroll
+    for (int q = 0; q < kWaves; q++) t += lds[q];
+    *total = t;
+    aim *= t;
+  }
+  int pick = -1; // the first wave that exceeds the aim; if rounding leaves none, the last with any mass
+  double before = 0.0, sum = 0.0;
+  for (int q = 0; q < kWaves; q++) {
+    const double v = lds[q];
+    if (v > 0.0) {
+      pick = q;
+      before = sum;
+      if (sum + v > aim) break;
+    }
+    sum += v;
+  }
+  int place = -1;
+  if (wave == pick) {
+    aim -= before;
+    sum = before = 0.0;
+    int at = -1;
+    double mine = 0.0;
+    bool done = false;
+#pragma unroll
+    for (int i = 0; i < VPT; i++) { // the same for the runs of 64
+      const double v = draw_wave_sum(w[i]);
+      if (!done && v > 0.0) {
+        at = i;
+        before = sum;
+        mine = w[i];
+        done = sum + v > aim;
+      }
+      sum += v;
+    }
+    aim -= before;
+    double run = mine;
+#pragma unroll
+    for (int d = 1; d < kWave; d <<= 1) {
+      const double b = __shfl_up(run, d);
+      if (lane >= d) run += b;
+    }
+    const unsigned long long over = __ballot(mine > 0.0 && run > aim), some = __ballot(mine > 0.0);
+    const int who = over ? __ffsll(over) - 1 : 63 - __clzll((long long)some);
+    if (lane == who) {
+      place = (wave * VPT + at) * kWave + lane;
+      *weight = mine;
+      *rest = aim - (run - mine);
+    }
+  }
+  return place;
+}
+
+// ---------------------------------------------------- whole rows, any data
+//
+// The key of the border is found eleven bits at a time, each time from a histogram over the whole row.  It needs nothing
+// of the data and serves the rows that the quick ways below hand back: more equal (or nearly equal) values at a border
+// than they have places for, a top-k of thousands.
+
 constexpr int kDrawBins = 2048;
 
 // What a workgroup shares.
@@ -78,33 +228,6 @@ template <typename T> struct DrawRow {
   __device__ __forceinline__ float at(int j) const { return (float)z[j]; }
   __device__ __forceinline__ bool kept(uint32_t k, int j) const { return k > key || (k == key && j <= last); }
 };
-
-// The row's largest value; *bad: it holds a NaN.
-template <typename T, int THREADS> __device__ float draw_row_max(const DrawRow<T> &r, DrawShared &s, bool *bad)
-{
-  float m = -HUGE_VALF;
-  bool nan = false;
-  for (int j = threadIdx.x; j < r.n; j += THREADS) {
-    const float z = r.at(j);
-    nan |= z != z;
-    m = fmaxf(m, z);
-  }
-#pragma unroll
-  for (int k = 1; k < kWave; k <<= 1) m = fmaxf(m, __shfl_xor(m, k));
-  const bool any = __any(nan);
-  if (threadIdx.x % kWave == 0) {
-    s.f[threadIdx.x / kWave] = m;
-    s.i[threadIdx.x / kWave] = any;
-  }
-  __syncthreads();
-  *bad = false;
-  for (int w = 0; w < THREADS / kWave; w++) {
-    m = fmaxf(m, s.f[w]);
-    *bad |= s.i[w] != 0;
-  }
-  __syncthreads();
-  return m;
-}
 
 // The prefix of the kept order that is needed for `k` values (BY_MASS false) or for `share` of the kept mass (true):
 // key and column are narrowed.  The key is found eleven bits at a time from a histogram of the values that share the
@@ -265,67 +388,816 @@ __device__ void draw_narrow(DrawRow<T> &r, DrawShared &s, int shift, uint32_t k,
   r.last = last;
 }
 
-// One workgroup a row.
-template <typename T, int THREADS> __global__ __launch_bounds__(THREADS) void draw_row_kernel(DrawArgs a, int shift)
+
+// ------------------------------------------------ rows that fit a workgroup
+//
+// The values stay in registers, 64 consecutive columns to a wave's register.  One histogram by distance from the largest
+// (counts and masses) gives the bin in which a border falls; the few values of that bin go to LDS and each finds its
+// rank, and the mass before it, by comparing with all others.
+
+constexpr int kShortBins = 1024;
+template <int THREADS> struct ShortShared {
+  static constexpr int kCap = THREADS; // values of a border's bin
+  unsigned long long mass[kShortBins];
+  uint32_t count[kShortBins];
+  unsigned long long place[kCap];
+  unsigned long long cmass[kCap];
+  double d[32];
+  unsigned long long q[32];
+  float f[32], g[32];
+  uint32_t i[32];
+};
+
+// Narrows the kept prefix.  z: -inf where there is nothing; column j of z[i] from at(i).  Returns false if a border's
+// bin holds more values than there is room for.
+template <int THREADS, int VPT, typename AT>
+__device__ bool draw_short_narrow(const float (&z)[VPT], AT at, float max, float min, const DrawChoice &c, int shift,
+                                  ShortShared<THREADS> &s, DrawEnd *end)
 {
-  __shared__ DrawShared s;
-  const int64_t row = blockIdx.x;
+  constexpr int kWaves = THREADS / kWave, kRun = kShortBins / THREADS;
   const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
-  constexpr int kWaves = THREADS / kWave;
+  const DrawBin<kShortBins> bin(max, min, c.temp);
+  const bool by_mass = c.share < 1.0;
+  const double unit = ldexp(1.0, -shift);
+  for (int b = tid; b < kShortBins; b += THREADS) {
+    s.count[b] = 0;
+    s.mass[b] = 0;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < VPT; i++)
+    if (z[i] > -HUGE_VALF) {
+      const int b = bin.of(z[i]);
+      atomicAdd(&s.count[b], 1u);
+      if (by_mass) {
+        const unsigned long long m = draw_fixed(draw_weight(z[i], max, c.inv_t), shift);
+        if (m) atomicAdd(&s.mass[b], m);
+      }
+    }
+  __syncthreads();
+  // sums before each bin; a thread has kRun bins
+  uint32_t cn = 0;
+  unsigned long long cm = 0;
+#pragma unroll
+  for (int i = 0; i < kRun; i++) {
+    cn += s.count[tid * kRun + i];
+    cm += s.mass[tid * kRun + i];
+  }
+  uint32_t in = cn;
+  unsigned long long im = cm;
+#pragma unroll
+  for (int d = 1; d < kWave; d <<= 1) {
+    const uint32_t a = __shfl_up(in, d);
+    const unsigned long long b = __shfl_up(im, d);
+    if (lane >= d) {
+      in += a;
+      im += b;
+    }
+  }
+  if (lane == kWave - 1) {
+    s.i[wave] = in;
+    s.q[wave] = im;
+  }
+  if (tid == 0) {
+    s.i[31] = kShortBins; // the bin of the top-k border
+    s.i[30] = 0;          // values gathered
+  }
+  __syncthreads();
+  uint32_t some = 0;
+  unsigned long long all = 0;
+#pragma unroll
+  for (int w = 0; w < kWaves; w++) {
+    if (w < wave) {
+      in += s.i[w];
+      im += s.q[w];
+    }
+    some += s.i[w];
+    all += s.q[w];
+  }
+  const bool by_count = c.k > 0 && (uint32_t)c.k < some;
+  unsigned long long place = ~0ull; // the last kept
+  int gathered = -1;
+  if (by_count) {
+    uint32_t n = in - cn;
+    unsigned long long m = im - cm;
+    for (int i = 0; i < kRun; i++) {
+      const uint32_t here = s.count[tid * kRun + i];
+      if (n < (uint32_t)c.k && n + here >= (uint32_t)c.k) {
+        s.i[31] = tid * kRun + i;
+        s.i[29] = n;
+        s.q[29] = m;
+      }
+      n += here;
+      m += s.mass[tid * kRun + i];
+    }
+    __syncthreads();
+    gathered = (int)s.i[31];
+  }
+  // Bring the values of bin `gathered` to LDS; *m: how many
+  auto gather = [&](int which) {
+#pragma unroll
+    for (int i = 0; i < VPT; i++)
+      if (z[i] > -HUGE_VALF && bin.of(z[i]) == which) {
+        const uint32_t q = atomicAdd(&s.i[30], 1u);
+        if (q < ShortShared<THREADS>::kCap) {
+          s.place[q] = draw_place(z[i], at(i));
+          s.cmass[q] = by_mass ? draw_fixed(draw_weight(z[i], max, c.inv_t), shift) : 0;
+        }
+      }
+    __syncthreads();
+    return (int)s.i[30];
+  };
+  int m = 0;
+  unsigned long long before = 0; // of this thread's value, in its bin
+  uint32_t rank = 0;
+  auto order = [&]() {
+    before = 0;
+    rank = 0;
+    if (tid < m) {
+      const unsigned long long mine = s.place[tid];
+      for (int q = 0; q < m; q++)
+        if (s.place[q] < mine) {
+          rank++;
+          before += s.cmass[q];
+        }
+    }
+  };
+  if (by_count) {
+    m = gather(gathered);
+    if (m > ShortShared<THREADS>::kCap) return false;
+    order();
+    if (tid < m && s.i[29] + rank == (uint32_t)c.k - 1) {
+      s.q[31] = s.place[tid];
+      s.q[30] = s.q[29] + before + s.cmass[tid];
+    }
+    __syncthreads();
+    place = s.q[31];
+    all = s.q[30];
+  }
+  if (by_mass) {
+    const double target = c.share * ((double)all * unit);
+    // the last value before which less than the target lies
+    __syncthreads();
+    if (tid == 0) {
+      s.i[31] = kShortBins;
+      s.q[31] = 0;
+    }
+    __syncthreads();
+    uint32_t n = in - cn;
+    unsigned long long below = im - cm;
+    for (int i = 0; i < kRun; i++) {
+      const uint32_t here = s.count[tid * kRun + i];
+      const unsigned long long hm = s.mass[tid * kRun + i];
+      const bool first = n == 0;
+      if (here && ((double)below * unit < target || first) && (double)(below + hm) * unit >= target) {
+        atomicMin(&s.i[31], (uint32_t)(tid * kRun + i));
+      }
+      n += here;
+      below += hm;
+    }
+    __syncthreads();
+    int which = (int)s.i[31];
+    if (by_count && which > gathered) which = gathered;
+    // what lies before that bin
+    if (which / kRun == tid) {
+      unsigned long long b = im - cm;
+      for (int i = 0; i < which % kRun; i++) b += s.mass[tid * kRun + i];
+      s.q[29] = b;
+    }
+    if (tid == 0 && which != gathered) s.i[30] = 0;
+    __syncthreads();
+    const unsigned long long base = s.q[29];
+    if (which != gathered) {
+      m = gather(which);
+      if (m > ShortShared<THREADS>::kCap) return false;
+      order();
+    }
+    if (tid < m) {
+      const unsigned long long mine = s.place[tid];
+      if (mine <= place && ((double)(base + before) * unit < target || (base == 0 && rank == 0))) atomicMax(&s.q[31], mine);
+    }
+    __syncthreads();
+    place = s.q[31];
+  }
+  end->place = place;
+  return true;
+}
+
+// What the kernels that finish a row keep in LDS: one of the two at a time.
+template <int THREADS> union RowShared {
+  ShortShared<THREADS> quick;
+  DrawShared whole;
+};
+
+// The whole-row way to the end of the kept prefix.
+template <typename T, int THREADS>
+__device__ DrawEnd draw_whole(const DrawArgs &a, int64_t row, const DrawChoice &c, float max, int shift, DrawShared &s)
+{
   DrawRow<T> r;
   r.z = (const T *)a.z + row * a.stride;
   r.n = (int)a.n;
-  const double temp = a.temperature ? (double)a.temperature[row] : a.temperature_all;
-  const double share = a.top_p ? (double)a.top_p[row] : a.top_p_all;
-  const double least = a.min_p ? (double)a.min_p[row] : a.min_p_all;
-  const int k = a.top_k ? a.top_k[row] : a.top_k_all;
-  const double u = a.u_is_double ? ((const double *)a.u)[row] : (double)((const float *)a.u)[row];
-  bool bad;
-  r.max = draw_row_max<T, THREADS>(r, s, &bad);
-  // nothing to draw: no weight, or a number that is none
-  if (bad || r.max == -HUGE_VALF || !(temp >= 0.0) || share != share || least != least || u != u) {
-    if (tid == 0) {
-      a.index[row] = -1;
-      if (a.logp) a.logp[row] = __uint_as_float(0x7fc00000u);
+  r.max = max;
+  r.inv_t = c.inv_t;
+  r.key = 0;
+  r.last = r.n;
+  __syncthreads();
+  if (c.k) draw_narrow<T, THREADS, false>(r, s, shift, (uint32_t)c.k, 0.0);
+  if (c.share < 1.0) draw_narrow<T, THREADS, true>(r, s, shift, 0u, c.share);
+  __syncthreads();
+  return DrawEnd{(unsigned long long)~r.key << 32 | (uint32_t)r.last};
+}
+
+// Rows of up to THREADS * VPT values.
+template <typename T, int THREADS, int VPT> __global__ __launch_bounds__(THREADS) void draw_short_kernel(DrawArgs a, int shift)
+{
+  __shared__ RowShared<THREADS> s;
+  constexpr int kWaves = THREADS / kWave;
+  const int64_t row = blockIdx.x;
+  const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave, n = (int)a.n;
+  const T *zp = (const T *)a.z + row * a.stride;
+  float z[VPT];
+  auto at = [&](int i) { return (wave * VPT + i) * kWave + lane; };
+  float max = -HUGE_VALF, min = HUGE_VALF;
+  bool nan = false;
+#pragma unroll
+  for (int i = 0; i < VPT; i++) {
+    z[i] = at(i) < n ? (float)zp[at(i)] : -HUGE_VALF;
+    nan |= z[i] != z[i];
+    max = fmaxf(max, z[i]);
+    if (z[i] > -HUGE_VALF) min = fminf(min, z[i]);
+  }
+  const DrawChoice c = draw_choice(a, row);
+#pragma unroll
+  for (int d = 1; d < kWave; d <<= 1) {
+    max = fmaxf(max, __shfl_xor(max, d));
+    min = fminf(min, __shfl_xor(min, d));
+  }
+  const bool any = __any(nan);
+  if (lane == 0) {
+    s.quick.f[wave] = max;
+    s.quick.g[wave] = min;
+    s.quick.i[wave] = any;
+  }
+  __syncthreads();
+  bool bad = c.bad;
+#pragma unroll
+  for (int w = 0; w < kWaves; w++) {
+    max = fmaxf(max, s.quick.f[w]);
+    min = fminf(min, s.quick.g[w]);
+    bad |= s.quick.i[w] != 0;
+  }
+  __syncthreads();
+  if (bad || max == -HUGE_VALF) {
+    if (tid == 0) draw_nothing(a, row);
+    return;
+  }
+  if (c.greedy) {
+    if (tid == 0) s.quick.i[0] = 0xffffffffu;
+    __syncthreads();
+    int first = n;
+#pragma unroll
+    for (int i = VPT - 1; i >= 0; i--)
+      if (z[i] == max) first = at(i);
+    if (first < n) atomicMin(&s.quick.i[0], (uint32_t)first);
+    __syncthreads();
+    if (tid == 0) draw_answer(a, row, s.quick.i[0], 0.0);
+    return;
+  }
+  DrawEnd end{~0ull};
+  if (c.k || c.share < 1.0)
+    if (!draw_short_narrow<THREADS, VPT>(z, at, max, min, c, shift, s.quick, &end)) end = draw_whole<T, THREADS>(a, row, c, max, shift, s.whole);
+  double w[VPT];
+#pragma unroll
+  for (int i = 0; i < VPT; i++) {
+    w[i] = z[i] > -HUGE_VALF && end.kept(z[i], at(i)) ? draw_weight(z[i], max, c.inv_t) : 0.0;
+    if (w[i] < c.least) w[i] = 0.0;
+  }
+  double total, weight, rest;
+  __syncthreads();
+  const int place = draw_pick<THREADS, VPT, true>(w, c.u, &total, &weight, &rest, s.quick.d);
+  if (place >= 0) draw_answer(a, row, place, log(weight / total));
+}
+
+// --------------------------------------------------------------- long rows
+//
+// A row is cut into units of 64 * VPT columns, one a wave, so that a few long rows fill the chip too.  Up to four kernels,
+// of which the host leaves out those that no row needs:
+//   top      each unit's largest value; for plain rows (no top-k, top-p, min-p) its mass too, relative to that value
+//   histo    top-k: how many values lie in each bin of distance from the row's largest; top-p: their masses
+//   collect  from the histogram the border's bin.  top-k: every value down to that bin goes to the unit's list (with
+//            their place in order); top-p: the bin's own values go there, the mass of what lies above is summed; min-p
+//            alone: the sum
+//   finish   one workgroup a row: the border among the listed values, the unit in which the kept mass exceeds u of the
+//            whole, the column in it.  A row whose lists are too long goes the whole-row way.
+
+constexpr int kLongBins = 2048;
+constexpr int kLongList = 2048;  // listed values of a row
+constexpr int kLongUnits = 1024; // units of a row: one a thread of the finishing workgroup
+
+struct LongPart {
+  float max, min; // min: of the values above -inf
+  int first;      // column of max
+  int nan;
+  double mass;    // of exp((z - max) / T), plain rows
+};
+
+enum { kRowNothing = 0, kRowGreedy, kRowPlain, kRowSums, kRowList, kRowNucleus };
+
+struct LongCell { // one row's border bin
+  int bin;
+  int too_long;
+  unsigned long long above;
+  double target;
+};
+
+struct LongCand {
+  float z;
+  int j;
+};
+
+struct LongSpace {
+  LongPart *part;           // [rows][units]
+  double *kept;             // [rows][units]
+  int *listed;              // [rows][units]
+  LongCand *list;           // [rows][units][unit / 2]
+  unsigned long long *histo; // [rows][kLongBins]
+  LongCell *cell;           // [rows]
+  int units, groups;        // per row: waves, workgroups of four
+};
+
+// What a row needs.
+__device__ inline int draw_kind(const DrawChoice &c, bool bad, float max)
+{
+  if (bad || c.bad || max == -HUGE_VALF) return kRowNothing;
+  if (c.greedy) return kRowGreedy;
+  if (c.k) return kRowList;
+  if (c.share < 1.0) return kRowNucleus;
+  return c.least > 0.0 ? kRowSums : kRowPlain;
+}
+
+// The row's largest and smallest value from its units'; every wave does it for itself.
+__device__ inline void draw_row_range(const LongPart *part, int units, float *max, float *min, bool *nan)
+{
+  float a = -HUGE_VALF, b = HUGE_VALF;
+  int bad = 0;
+  for (int q = threadIdx.x % kWave; q < units; q += kWave) {
+    a = fmaxf(a, part[q].max);
+    b = fminf(b, part[q].min);
+    bad |= part[q].nan;
+  }
+#pragma unroll
+  for (int d = 1; d < kWave; d <<= 1) {
+    a = fmaxf(a, __shfl_xor(a, d));
+    b = fminf(b, __shfl_xor(b, d));
+  }
+  *max = a;
+  *min = b;
+  *nan = __any(bad) != 0;
+}
+
+// A unit's values: register v * VEC + e of lane l holds column base + (v * 64 + l) * VEC + e; -inf past the end.
+template <typename T, int VEC, int VPT> __device__ __forceinline__ void draw_load(const T *row, int n, int base, float (&z)[VPT])
+{
+  struct alignas(sizeof(T) * VEC) Pack { T e[VEC]; };
+  const int lane = threadIdx.x % kWave;
+  if (base + VPT * kWave <= n) {
+    Pack p[VPT / VEC];
+#pragma unroll
+    for (int v = 0; v < VPT / VEC; v++) p[v] = *(const Pack *)(row + base + (v * kWave + lane) * VEC);
+#pragma unroll
+    for (int v = 0; v < VPT / VEC; v++)
+#pragma unroll
+      for (int e = 0; e < VEC; e++) z[v * VEC + e] = (float)p[v].e[e];
+  } else {
+#pragma unroll
+    for (int v = 0; v < VPT / VEC; v++)
+#pragma unroll
+      for (int e = 0; e < VEC; e++) {
+        const int j = base + (v * kWave + lane) * VEC + e;
+        z[v * VEC + e] = j < n ? (float)row[j] : -HUGE_VALF;
+      }
+  }
+}
+template <int VEC> __device__ __forceinline__ int draw_column(int base, int i)
+{
+  return base + (i / VEC * kWave + (int)threadIdx.x % kWave) * VEC + i % VEC;
+}
+
+template <typename T, int VEC, int VPT>
+__global__ __launch_bounds__(kBlock) void draw_top_kernel(DrawArgs a, LongSpace g, int with_histo)
+{
+  const int64_t row = blockIdx.x / g.groups;
+  const int group = blockIdx.x % g.groups, wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
+  if (with_histo)
+    for (int b = group * kBlock + threadIdx.x; b < kLongBins; b += g.groups * kBlock) g.histo[row * kLongBins + b] = 0;
+  const int unit = group * 4 + wave;
+  if (unit >= g.units) return;
+  const int base = unit * VPT * kWave;
+  float z[VPT];
+  draw_load<T, VEC, VPT>((const T *)a.z + row * a.stride, (int)a.n, base, z);
+  float max = -HUGE_VALF, min = HUGE_VALF;
+  bool nan = false;
+#pragma unroll
+  for (int i = 0; i < VPT; i++) {
+    nan |= z[i] != z[i];
+    max = fmaxf(max, z[i]);
+    if (z[i] > -HUGE_VALF) min = fminf(min, z[i]);
+  }
+#pragma unroll
+  for (int d = 1; d < kWave; d <<= 1) {
+    max = fmaxf(max, __shfl_xor(max, d));
+    min = fminf(min, __shfl_xor(min, d));
+  }
+  const DrawChoice c = draw_choice(a, row);
+  int first = INT32_MAX;
+  double mass = 0.0;
+  if (c.greedy) {
+#pragma unroll
+    for (int i = VPT - 1; i >= 0; i--)
+      if (z[i] == max) first = draw_column<VEC>(base, i);
+#pragma unroll
+    for (int d = 1; d < kWave; d <<= 1) {
+      const int o = __shfl_xor(first, d);
+      first = o < first ? o : first;
+    }
+  } else if (draw_kind(c, false, max) == kRowPlain) {
+#pragma unroll
+    for (int i = 0; i < VPT; i++) mass += draw_weight(z[i], max, c.inv_t);
+    mass = draw_wave_sum(mass);
+  }
+  const bool any = __any(nan);
+  if (lane == 0) g.part[row * g.units + unit] = LongPart{max, min, first, any, mass};
+}
+
+template <typename T, int VEC, int VPT>
+__global__ __launch_bounds__(kBlock) void draw_histo_kernel(DrawArgs a, LongSpace g, int shift)
+{
+  __shared__ unsigned long long bins[kLongBins];
+  const int64_t row = blockIdx.x / g.groups;
+  const int group = blockIdx.x % g.groups, wave = threadIdx.x / kWave;
+  float max, min;
+  bool nan;
+  draw_row_range(g.part + row * g.units, g.units, &max, &min, &nan);
+  const DrawChoice c = draw_choice(a, row);
+  const int kind = draw_kind(c, nan, max);
+  if (kind != kRowList && kind != kRowNucleus) return;
+  for (int b = threadIdx.x; b < kLongBins; b += kBlock) bins[b] = 0;
+  __syncthreads();
+  const DrawBin<kLongBins> bin(max, min, c.temp);
+  const int unit = group * 4 + wave;
+  if (unit < g.units) {
+    float z[VPT];
+    draw_load<T, VEC, VPT>((const T *)a.z + row * a.stride, (int)a.n, unit * VPT * kWave, z);
+#pragma unroll
+    for (int i = 0; i < VPT; i++)
+      if (z[i] > -HUGE_VALF) {
+        const unsigned long long m = kind == kRowList ? 1 : draw_fixed(draw_weight(z[i], max, c.inv_t), shift);
+        if (m) atomicAdd(&bins[bin.of(z[i])], m);
+      }
+  }
+  __syncthreads();
+  for (int b = threadIdx.x; b < kLongBins; b += kBlock)
+    if (bins[b]) atomicAdd(&g.histo[row * kLongBins + b], bins[b]);
+}
+
+template <typename T, int VEC, int VPT>
+__global__ __launch_bounds__(kBlock) void draw_collect_kernel(DrawArgs a, LongSpace g, int shift)
+{
+  __shared__ unsigned long long sums[kBlock / kWave];
+  __shared__ LongCell cell;
+  const int64_t row = blockIdx.x / g.groups;
+  const int tid = threadIdx.x, group = blockIdx.x % g.groups, wave = tid / kWave, lane = tid % kWave;
+  float max, min;
+  bool nan;
+  draw_row_range(g.part + row * g.units, g.units, &max, &min, &nan);
+  const DrawChoice c = draw_choice(a, row);
+  const int kind = draw_kind(c, nan, max);
+  if (kind < kRowSums) return;
+  int border = kLongBins; // first bin that is listed (nucleus), or first that is not (list)
+  bool too_long = false;
+  if (kind != kRowSums) {
+    constexpr int kRun = kLongBins / kBlock;
+    unsigned long long h[kRun], mine = 0;
+#pragma unroll
+    for (int i = 0; i < kRun; i++) {
+      h[i] = g.histo[row * kLongBins + tid * kRun + i];
+      mine += h[i];
+    }
+    unsigned long long in = mine;
+#pragma unroll
+    for (int d = 1; d < kWave; d <<= 1) {
+      const unsigned long long b = __shfl_up(in, d);
+      if (lane >= d) in += b;
+    }
+    if (lane == kWave - 1) sums[wave] = in;
+    if (tid == 0) cell = LongCell{kLongBins - 1, 0, 0, 0.0};
+    __syncthreads();
+    unsigned long long all = 0;
+#pragma unroll
+    for (int w = 0; w < kBlock / kWave; w++) {
+      if (w < wave) in += sums[w];
+      all += sums[w];
+    }
+    const double unit = ldexp(1.0, -shift), target = kind == kRowNucleus ? c.share * ((double)all * unit) : 0.0;
+    unsigned long long before = in - mine;
+#pragma unroll
+    for (int i = 0; i < kRun; i++) {
+      const unsigned long long after = before + h[i];
+      const bool here = kind == kRowList ? before < (unsigned long long)c.k && after >= (unsigned long long)c.k
+                                         : h[i] && ((double)before * unit < target || before == 0) && (double)after * unit >= target;
+      if (here) cell = LongCell{tid * kRun + i, kind == kRowList && after > kLongList, before, target};
+      before = after;
+    }
+    if (kind == kRowList && tid == 0 && all < (unsigned long long)c.k) cell.too_long = all > kLongList; // fewer values than k: all
+    __syncthreads();
+    border = cell.bin;
+    too_long = cell.too_long;
+    if (group == 0 && tid == 0) g.cell[row] = cell;
+  }
+  const int u = group * 4 + wave;
+  if (u >= g.units || too_long) return;
+  constexpr int kUnit = VPT * kWave;
+  float z[VPT];
+  draw_load<T, VEC, VPT>((const T *)a.z + row * a.stride, (int)a.n, u * kUnit, z);
+  const DrawBin<kLongBins> bin(max, min, c.temp);
+  double kept = 0.0;
+  int n = 0;
+  LongCand *list = g.list + (row * g.units + u) * (kUnit / 2);
+#pragma unroll
+  for (int v = 0; v < VPT / VEC; v++) {
+    bool take[VEC];
+    int earlier = 0, total = 0; // of the same columns in lower lanes; of all lanes
+#pragma unroll
+    for (int e = 0; e < VEC; e++) {
+      const float x = z[v * VEC + e];
+      take[e] = false;
+      if (kind == kRowSums) {
+        const double w = draw_weight(x, max, c.inv_t);
+        if (w >= c.least) kept += w;
+      } else if (x > -HUGE_VALF) {
+        const int b = bin.of(x);
+        take[e] = kind == kRowList ? b <= border : b == border;
+        if (kind == kRowNucleus && b < border) {
+          const double w = draw_weight(x, max, c.inv_t);
+          if (w >= c.least) kept += w;
+        }
+      }
+      const unsigned long long t = __ballot(take[e]);
+      earlier += __popcll(t & ((1ull << lane) - 1));
+      total += __popcll(t);
+    }
+#pragma unroll
+    for (int e = 0; e < VEC; e++)
+      if (take[e]) {
+        const int q = n + earlier++;
+        if (q < kUnit / 2) list[q] = LongCand{z[v * VEC + e], draw_column<VEC>(u * kUnit, v * VEC + e)};
+      }
+    n += total;
+  }
+  kept = draw_wave_sum(kept);
+  if (lane == 0) {
+    g.kept[row * g.units + u] = kept;
+    g.listed[row * g.units + u] = n;
+  }
+}
+
+// One workgroup of 1024 a row.
+template <typename T, int VPT> __global__ __launch_bounds__(1024) void draw_finish_kernel(DrawArgs a, LongSpace g, int shift)
+{
+  constexpr int kThreads = 1024, kUnit = VPT * kWave, kIn = (kUnit + kThreads - 1) / kThreads;
+  __shared__ RowShared<kThreads> s;
+  __shared__ LongCand list[kLongList];
+  __shared__ int from[kLongUnits]; // where a unit's list begins
+  __shared__ int chosen;
+  __shared__ double left;
+  const int64_t row = blockIdx.x;
+  const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
+  const LongPart *part = g.part + row * g.units;
+  float max, min;
+  bool nan;
+  draw_row_range(part, g.units, &max, &min, &nan);
+  const DrawChoice c = draw_choice(a, row);
+  const int kind = draw_kind(c, nan, max);
+  if (kind == kRowNothing) {
+    if (tid == 0) draw_nothing(a, row);
+    return;
+  }
+  if (kind == kRowGreedy) {
+    if (wave == 0) {
+      int first = INT32_MAX;
+      for (int q = lane; q < g.units; q += kWave)
+        if (part[q].max == max && part[q].first < first) first = part[q].first;
+#pragma unroll
+      for (int d = 1; d < kWave; d <<= 1) {
+        const int o = __shfl_xor(first, d);
+        first = o < first ? o : first;
+      }
+      if (lane == 0) draw_answer(a, row, first, 0.0);
     }
     return;
   }
-  r.key = 0;
-  r.last = r.n;
-  const bool greedy = temp == 0.0;
-  r.inv_t = greedy ? 1.0 : 1.0 / temp;
-  if (greedy)
-    draw_narrow<T, THREADS, false>(r, s, shift, 1u, 0.0);
-  else {
-    if (k > 0 && k < r.n) draw_narrow<T, THREADS, false>(r, s, shift, (uint32_t)k, 0.0);
-    if (share < 1.0) draw_narrow<T, THREADS, true>(r, s, shift, 0u, share > 0.0 ? share : 0.0);
-  }
-  const double least1 = least > 1.0 ? 1.0 : least;
-  auto weight = [&](int j) {
-    const float z = r.at(j);
-    if (!r.kept(draw_key(z), j)) return 0.0;
-    const double w = draw_weight(z, r.max, r.inv_t);
-    return w >= least1 ? w : 0.0;
-  };
-
-  // Runs of columns, one a wave; then the run in which the kept mass exceeds u of it is cut into runs again.
-  int from = 0, to = r.n;
-  double total = 0.0, aim = 0.0;
-  for (bool first = true; first || to - from > kWave; first = false) {
-    const int run = ((to - from + kWaves - 1) / kWaves + kWave - 1) / kWave * kWave;
-    const int lo = from + wave * run < to ? from + wave * run : to, hi = lo + run < to ? lo + run : to;
-    double m = 0.0;
-    for (int j = lo + lane; j < hi; j += kWave) m += weight(j);
+  DrawEnd end{~0ull};
+  bool whole = false;
+  int listed = 0;
+  LongCell cell{0, 0, 0, 0.0};
+  if (kind >= kRowList) {
+    cell = g.cell[row];
+    whole = cell.too_long != 0;
+    int mine = 0, in = 0;
+    if (!whole) {
+      mine = tid < g.units ? g.listed[row * g.units + tid] : 0;
+      if (mine > kUnit / 2) mine = kLongList + 1; // the unit's list is too short
+      in = mine;
 #pragma unroll
-    for (int d = 1; d < kWave; d <<= 1) m += __shfl_xor(m, d);
+      for (int d = 1; d < kWave; d <<= 1) {
+        const int b = __shfl_up(in, d);
+        if (lane >= d) in += b;
+      }
+      if (lane == kWave - 1) s.quick.i[wave] = (uint32_t)in;
+      __syncthreads();
+      for (int w = 0; w < kThreads / kWave; w++) {
+        if (w < wave) in += (int)s.quick.i[w];
+        listed += (int)s.quick.i[w];
+      }
+      if (tid < g.units) from[tid] = in - mine;
+      __syncthreads();
+      whole = listed > (kind == kRowList ? kLongList : kThreads);
+    }
+    if (!whole) { // a wave brings a unit's list
+      for (int q = wave; q < g.units; q += kThreads / kWave) {
+        const int n = g.listed[row * g.units + q];
+        const LongCand *l = g.list + (row * g.units + q) * (kUnit / 2);
+        for (int i = lane; i < n; i += kWave) list[from[q] + i] = l[i];
+      }
+      __syncthreads();
+    }
+  }
+  if (kind == kRowList && !whole) {
+    constexpr int kList = kLongList / kThreads;
+    float z[kList];
+    auto place_of = [&](int i) { return (wave * kList + i) * kWave + lane; };
+    auto at = [&](int i) { return list[place_of(i)].j; };
+#pragma unroll
+    for (int i = 0; i < kList; i++) z[i] = place_of(i) < listed ? list[place_of(i)].z : -HUGE_VALF;
+    if (draw_short_narrow<kThreads, kList>(z, at, max, min, c, shift, s.quick, &end)) {
+      double w[kList];
+#pragma unroll
+      for (int i = 0; i < kList; i++) {
+        w[i] = z[i] > -HUGE_VALF && end.kept(z[i], at(i)) ? draw_weight(z[i], max, c.inv_t) : 0.0;
+        if (w[i] < c.least) w[i] = 0.0;
+      }
+      double total, weight, rest;
+      __syncthreads();
+      const int place = draw_pick<kThreads, kList, true>(w, c.u, &total, &weight, &rest, s.quick.d);
+      if (place >= 0) draw_answer(a, row, list[place].j, log(weight / total));
+      return;
+    }
+    whole = true;
+  }
+  const T *zp = (const T *)a.z + row * a.stride;
+  const int n = (int)a.n;
+  if (whole) end = draw_whole<T, kThreads>(a, row, c, max, shift, s.whole);
+  if (kind == kRowNucleus && !whole) { // the border among the listed
+    unsigned long long *mass = s.quick.cmass, *place = s.quick.place;
+    const double unit = ldexp(1.0, -shift);
+    if (tid < listed) {
+      mass[tid] = draw_fixed(draw_weight(list[tid].z, max, c.inv_t), shift);
+      place[tid] = draw_place(list[tid].z, list[tid].j);
+    }
+    if (tid == 0) s.quick.q[31] = 0;
+    __syncthreads();
+    if (tid < listed) {
+      const unsigned long long mine = place[tid];
+      unsigned long long before = cell.above;
+      int rank = 0;
+      for (int q = 0; q < listed; q++)
+        if (place[q] < mine) {
+          before += mass[q];
+          rank++;
+        }
+      if ((double)before * unit < cell.target || (cell.above == 0 && rank == 0)) atomicMax(&s.quick.q[31], mine);
+    }
+    __syncthreads();
+    end.place = s.quick.q[31];
+  }
+  // The kept mass of each unit
+  auto weight_of = [&](float z, int j) {
+    const double w = z > -HUGE_VALF && end.kept(z, j) ? draw_weight(z, max, c.inv_t) : 0.0;
+    return w >= c.least ? w : 0.0;
+  };
+  double m[1] = {0.0};
+  if (whole) {
+    for (int q = wave; q < g.units; q += kThreads / kWave) {
+      double v = 0.0;
+      for (int i = 0; i < VPT; i++) {
+        const int j = q * kUnit + i * kWave + lane;
+        if (j < n) v += weight_of((float)zp[j], j);
+      }
+      v = draw_wave_sum(v);
+      if (lane == 0) g.kept[row * g.units + q] = v;
+    }
+    __threadfence_block();
+    __syncthreads();
+  }
+  if (tid < g.units) {
+    if (kind == kRowPlain)
+      m[0] = part[tid].mass * draw_weight(part[tid].max, max, c.inv_t);
+    else {
+      m[0] = g.kept[row * g.units + tid];
+      if (kind == kRowNucleus && !whole)
+        for (int q = from[tid], to = tid + 1 < g.units ? from[tid + 1] : listed; q < to; q++) m[0] += weight_of(list[q].z, list[q].j);
+    }
+  }
+  double total = 0.0, weight, rest;
+  __syncthreads();
+  const int unit = draw_pick<kThreads, 1, true>(m, c.u, &total, &weight, &rest, s.quick.d);
+  if (unit >= 0) {
+    chosen = unit;
+    left = rest;
+  }
+  __syncthreads();
+  // ... and the column in the unit
+  const int base = chosen * kUnit;
+  const double aim = left;
+  double w[kIn];
+#pragma unroll
+  for (int i = 0; i < kIn; i++) {
+    const int q = (wave * kIn + i) * kWave + lane, j = base + q;
+    w[i] = q < kUnit && j < n ? weight_of((float)zp[j], j) : 0.0;
+  }
+  double ignored;
+  const int place = draw_pick<kThreads, kIn, false>(w, aim, &ignored, &weight, &rest, s.quick.d);
+  if (place >= 0) draw_answer(a, row, base + place, log(weight / total));
+}
+
+// Rows too long for the units: one workgroup a row, whole-row ways only.
+template <typename T> __global__ __launch_bounds__(1024) void draw_huge_kernel(DrawArgs a, int shift)
+{
+  constexpr int kThreads = 1024, kWaves = kThreads / kWave;
+  __shared__ DrawShared s;
+  __shared__ uint32_t first;
+  const int64_t row = blockIdx.x;
+  const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave, n = (int)a.n;
+  const T *zp = (const T *)a.z + row * a.stride;
+  const DrawChoice c = draw_choice(a, row);
+  float max = -HUGE_VALF;
+  bool nan = false;
+  for (int j = tid; j < n; j += kThreads) {
+    const float z = (float)zp[j];
+    nan |= z != z;
+    max = fmaxf(max, z);
+  }
+#pragma unroll
+  for (int d = 1; d < kWave; d <<= 1) max = fmaxf(max, __shfl_xor(max, d));
+  const bool any = __any(nan);
+  if (lane == 0) {
+    s.f[wave] = max;
+    s.i[wave] = any;
+  }
+  if (tid == 0) first = 0xffffffffu;
+  __syncthreads();
+  bool bad = c.bad;
+  for (int w = 0; w < kWaves; w++) {
+    max = fmaxf(max, s.f[w]);
+    bad |= s.i[w] != 0;
+  }
+  __syncthreads();
+  if (bad || max == -HUGE_VALF) {
+    if (tid == 0) draw_nothing(a, row);
+    return;
+  }
+  if (c.greedy) {
+    for (int j = tid; j < n; j += kThreads)
+      if ((float)zp[j] == max) {
+        atomicMin(&first, (uint32_t)j);
+        break;
+      }
+    __syncthreads();
+    if (tid == 0) draw_answer(a, row, first, 0.0);
+    return;
+  }
+  const DrawEnd end = draw_whole<T, kThreads>(a, row, c, max, shift, s);
+  auto weight_of = [&](int j) {
+    const float z = (float)zp[j];
+    const double w = z > -HUGE_VALF && end.kept(z, j) ? draw_weight(z, max, c.inv_t) : 0.0;
+    return w >= c.least ? w : 0.0;
+  };
+  // Runs of columns, one a wave; then the run in which the kept mass exceeds u of it is cut into runs again.
+  int64_t from = 0, to = n;
+  double total = 0.0, aim = 0.0;
+  for (bool start = true; start || to - from > kWave; start = false) {
+    const int64_t run = ((to - from + kWaves - 1) / kWaves + kWave - 1) / kWave * kWave;
+    const int64_t lo = from + wave * run < to ? from + wave * run : to, hi = lo + run < to ? lo + run : to;
+    double m = 0.0;
+    for (int64_t j = lo + lane; j < hi; j += kWave) m += weight_of((int)j);
+    m = draw_wave_sum(m);
     __syncthreads();
     if (lane == 0) s.d[wave] = m;
     __syncthreads();
-    if (first) {
+    if (start) {
       for (int w = 0; w < kWaves; w++) total += s.d[w];
-      aim = u * total;
+      aim = c.u * total;
     }
-    // the first run that exceeds the aim; if rounding leaves none, the last one with any mass
     int pick = -1;
     double before = 0.0, sum = 0.0;
     for (int w = 0; w < kWaves; w++) {
@@ -342,7 +1214,7 @@ template <typename T, int THREADS> __global__ __launch_bounds__(THREADS) void dr
     to = from + run < to ? from + run : to;
   }
   if (wave == 0) {
-    const double w = lane < to - from ? weight(from + lane) : 0.0;
+    const double w = lane < to - from ? weight_of((int)from + lane) : 0.0;
     double m = w;
 #pragma unroll
     for (int d = 1; d < kWave; d <<= 1) {
@@ -350,11 +1222,8 @@ template <typename T, int THREADS> __global__ __launch_bounds__(THREADS) void dr
       if (lane >= d) m += b;
     }
     const unsigned long long over = __ballot(w > 0.0 && m > aim), some = __ballot(w > 0.0);
-    const int pick = over ? __ffsll((unsigned long long)over) - 1 : 63 - __clzll(some);
-    if (lane == pick) {
-      a.index[row] = from + lane;
-      if (a.logp) a.logp[row] = greedy ? 0.f : (float)log(w / total);
-    }
+    const int pick = over ? __ffsll(over) - 1 : 63 - __clzll((long long)some);
+    if (lane == pick) draw_answer(a, row, from + lane, log(w / total));
   }
 }
 

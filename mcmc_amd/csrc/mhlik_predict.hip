@@ -145,15 +145,96 @@ template <typename T> int product_launch(Q8Product a, hipStream_t stream)
   return MHLIK_OK;
 }
 
-template <typename T> int draw_launch(const DrawArgs &a, hipStream_t stream)
+// How a batch of rows is drawn from.
+struct DrawPlan {
+  int vpt = 0;     // long rows: values a lane of a unit holds; 0: rows that fit a workgroup, or too long for units
+  bool short_rows = false;
+  LongSpace space;
+  size_t bytes = 0;
+};
+
+constexpr int kShortMax = 8192;  // columns that fit a workgroup's registers (1024 threads, 8 each)
+constexpr int64_t kLongVpt = 32; // a unit: 2048 columns; 512 where those would leave the chip's 1024 SIMDs idle
+
+DrawPlan draw_plan(int64_t rows, int64_t n, void *workspace)
 {
-  int shift = 63;
+  DrawPlan p;
+  p.short_rows = n <= kShortMax;
+  if (p.short_rows) return p;
+  p.vpt = rows * ((n + kLongVpt * kWave - 1) / (kLongVpt * kWave)) < 2048 && n <= (int64_t)8 * kWave * kLongUnits ? 8 : kLongVpt;
+  const int64_t unit = p.vpt * kWave, units = (n + unit - 1) / unit;
+  if (units > kLongUnits) {
+    p.vpt = 0;
+    return p;
+  }
+  LongSpace &g = p.space;
+  g.units = (int)units;
+  g.groups = (int)((units + 3) / 4);
+  uint8_t *at = (uint8_t *)workspace;
+  auto take = [&](size_t bytes) {
+    uint8_t *q = at ? at + p.bytes : nullptr;
+    p.bytes += (bytes + 63) / 64 * 64;
+    return q;
+  };
+  g.part = (LongPart *)take(sizeof(LongPart) * rows * units);
+  g.kept = (double *)take(sizeof(double) * rows * units);
+  g.listed = (int *)take(sizeof(int) * rows * units);
+  g.histo = (unsigned long long *)take(sizeof(unsigned long long) * rows * kLongBins);
+  g.cell = (LongCell *)take(sizeof(LongCell) * rows);
+  g.list = (LongCand *)take(sizeof(LongCand) * rows * units * (unit / 2));
+  return p;
+}
+
+template <typename T, int VEC, int VPT> void draw_long(const DrawArgs &a, const LongSpace &g, int shift, bool histo, bool collect, hipStream_t stream)
+{
+  const dim3 grid((unsigned)(a.rows * g.groups));
+  hipLaunchKernelGGL((draw_top_kernel<T, VEC, VPT>), grid, dim3(kBlock), 0, stream, a, g, (int)histo);
+  if (histo) hipLaunchKernelGGL((draw_histo_kernel<T, VEC, VPT>), grid, dim3(kBlock), 0, stream, a, g, shift);
+  if (collect) hipLaunchKernelGGL((draw_collect_kernel<T, VEC, VPT>), grid, dim3(kBlock), 0, stream, a, g, shift);
+  hipLaunchKernelGGL((draw_finish_kernel<T, VPT>), dim3((unsigned)a.rows), dim3(1024), 0, stream, a, g, shift);
+}
+
+template <typename T> int draw_launch(const DrawArgs &a, void *workspace, size_t workspace_bytes, hipStream_t stream)
+{
+  int shift = 63; // weights in whole numbers: n of them stay below 2^63
   while (((int64_t)1 << (63 - shift)) < a.n) shift--;
-  if (a.n <= 4096)
-    hipLaunchKernelGGL((draw_row_kernel<T, 256>), dim3((unsigned)a.rows), dim3(256), 0, stream, a, shift);
-  else
-    hipLaunchKernelGGL((draw_row_kernel<T, 1024>), dim3((unsigned)a.rows), dim3(1024), 0, stream, a, shift);
+  const DrawPlan p = draw_plan(a.rows, a.n, workspace);
+  if (p.bytes && (!aligned16(workspace) || !workspace || workspace_bytes < p.bytes))
+    return fail_no_ctx(MHLIK_EINVAL, "workspace: %zu bytes at a multiple of 16 are needed (%zu given)", p.bytes, workspace_bytes);
+  if (p.short_rows) {
+    const dim3 grid((unsigned)a.rows);
+    if (a.n <= 512)
+      hipLaunchKernelGGL((draw_short_kernel<T, 256, 2>), grid, dim3(256), 0, stream, a, shift);
+    else if (a.n <= 2048)
+      hipLaunchKernelGGL((draw_short_kernel<T, 256, 8>), grid, dim3(256), 0, stream, a, shift);
+    else
+      hipLaunchKernelGGL((draw_short_kernel<T, 1024, 8>), grid, dim3(1024), 0, stream, a, shift);
+  } else if (!p.vpt) {
+    hipLaunchKernelGGL(draw_huge_kernel<T>, dim3((unsigned)a.rows), dim3(1024), 0, stream, a, shift);
+  } else {
+    if (a.rows * p.space.groups > INT32_MAX)
+      return fail_no_ctx(MHLIK_EINVAL, "too many rows of this length (%lld x %lld)", (long long)a.rows, (long long)a.n);
+    const bool histo = a.top_k || a.top_p || (a.top_k_all > 0 && a.top_k_all < a.n) || a.top_p_all < 1.0;
+    const bool collect = histo || a.min_p || a.min_p_all > 0.0;
+    constexpr int kVec = 16 / sizeof(T);
+    const bool vec = aligned16(a.z) && (a.rows == 1 || a.stride * (int64_t)sizeof(T) % 16 == 0);
+    if (p.vpt == 8 && vec)
+      draw_long<T, kVec, 8>(a, p.space, shift, histo, collect, stream);
+    else if (p.vpt == 8)
+      draw_long<T, 1, 8>(a, p.space, shift, histo, collect, stream);
+    else if (vec)
+      draw_long<T, kVec, kLongVpt>(a, p.space, shift, histo, collect, stream);
+    else
+      draw_long<T, 1, kLongVpt>(a, p.space, shift, histo, collect, stream);
+  }
   PCHK(hipGetLastError());
+  return MHLIK_OK;
+}
+
+int check_draw_shape(int64_t rows, int64_t n)
+{
+  if (rows < 0 || rows > INT32_MAX || n < 1 || n >= (int64_t)1 << 30)
+    return fail_no_ctx(MHLIK_EINVAL, "need 0 <= rows < 2^31 and 1 <= n < 2^30 (rows=%lld n=%lld)", (long long)rows, (long long)n);
   return MHLIK_OK;
 }
 
@@ -230,11 +311,18 @@ int mhlik_q8_product(const mhlik_q8_operands *p, int32_t device, void *stream)
   }
 }
 
+int mhlik_draw_workspace(int64_t rows, int64_t n, size_t *bytes)
+{
+  if (!bytes) return fail_no_ctx(MHLIK_EINVAL, "bytes must not be NULL");
+  if (int rc = check_draw_shape(rows, n)) return rc;
+  *bytes = draw_plan(rows, n, nullptr).bytes;
+  return MHLIK_OK;
+}
+
 int mhlik_draw(const mhlik_draw_rows *p, int32_t device, void *stream)
 {
   if (!p) return fail_no_ctx(MHLIK_EINVAL, "rows must not be NULL");
-  if (p->rows < 0 || p->rows > INT32_MAX || p->n < 1 || p->n >= INT32_MAX / 2)
-    return fail_no_ctx(MHLIK_EINVAL, "need 0 <= rows < 2^31 and 1 <= n < 2^30 (rows=%lld n=%lld)", (long long)p->rows, (long long)p->n);
+  if (int rc = check_draw_shape(p->rows, p->n)) return rc;
   if (p->z_type != MHLIK_T_F32 && p->z_type != MHLIK_T_BF16 && p->z_type != MHLIK_T_F16)
     return fail_no_ctx(MHLIK_EINVAL, "z: unknown element type %d", p->z_type);
   if (p->u_type != MHLIK_T_F64 && p->u_type != MHLIK_T_F32) return fail_no_ctx(MHLIK_EINVAL, "u: unknown element type %d", p->u_type);
@@ -265,9 +353,9 @@ int mhlik_draw(const mhlik_draw_rows *p, int32_t device, void *stream)
   a.index = p->index;
   a.logp = p->logp;
   switch (p->z_type) {
-  case MHLIK_T_F32: return draw_launch<float>(a, (hipStream_t)stream);
-  case MHLIK_T_BF16: return draw_launch<__bf16>(a, (hipStream_t)stream);
-  default: return draw_launch<_Float16>(a, (hipStream_t)stream);
+  case MHLIK_T_F32: return draw_launch<float>(a, p->workspace, p->workspace_bytes, (hipStream_t)stream);
+  case MHLIK_T_BF16: return draw_launch<__bf16>(a, p->workspace, p->workspace_bytes, (hipStream_t)stream);
+  default: return draw_launch<_Float16>(a, p->workspace, p->workspace_bytes, (hipStream_t)stream);
   }
 }
 }

@@ -168,5 +168,10 @@ def draw(z, u, temperature=1.0, top_k=None, top_p=None, min_p=None):
     p.z, p.rows, p.n, p.stride, p.z_type = z.data_ptr(), rows, n, z.stride(0), _OUT[z.dtype]
     p.u, p.u_type = u.data_ptr(), _U[u.dtype]
     p.index, p.logp = index.data_ptr(), logp.data_ptr()
+    need = C.c_size_t()
+    _chk(L.load_mhlik().mhlik_draw_workspace(rows, n, C.byref(need)))
+    if need.value:
+        space = torch.empty(need.value, dtype=torch.uint8, device=device)
+        p.workspace, p.workspace_bytes = space.data_ptr(), need.value
     _chk(L.load_mhlik().mhlik_draw(C.byref(p), device.index, _stream(device)))
     return index, logp
