@@ -10,6 +10,8 @@
 // above -96 so that q 2^k is a normal bfloat16, which the wide product needs.
 #pragma once
 
+#include <type_traits>
+
 #include "mhlik_predict.hpp"
 
 namespace mhlik {
@@ -19,12 +21,11 @@ constexpr int kQ8Lane = 8;        // columns a lane packs in the row kernel
 constexpr int kQ8MinExp = -96, kQ8MaxExp = 119;
 
 typedef float q8_f4 __attribute__((ext_vector_type(4)));
+typedef float q8_f16 __attribute__((ext_vector_type(16)));
 typedef int q8_i4 __attribute__((ext_vector_type(4)));
 typedef int q8_i8 __attribute__((ext_vector_type(8)));
 typedef __bf16 q8_b2 __attribute__((ext_vector_type(2)));
-typedef __bf16 q8_b4 __attribute__((ext_vector_type(4)));
 typedef __bf16 q8_b8 __attribute__((ext_vector_type(8)));
-typedef _Float16 q8_h4 __attribute__((ext_vector_type(4)));
 
 __host__ __device__ inline int64_t q8_blocks(int64_t cols) { return (cols + kQ8Block - 1) / kQ8Block; }
 __host__ __device__ inline int64_t q8_scale_stride(int64_t cols) { return (q8_blocks(cols) + 3) / 4 * 4; }
@@ -185,18 +186,27 @@ __device__ __forceinline__ q8_b8 q8_widen(q8_i8 v, int s, float scale)
 
 template <typename T> __device__ __forceinline__ T q8_round(float v) { return (T)v; }
 
-// Four consecutive values of a row of C.
-template <typename T> __device__ __forceinline__ void q8_store4(T *p, q8_f4 v, int n, bool aligned)
+// Values that go to or come from any address of their type in one access: gfx950 takes unaligned ones, an access that
+// spans two lines costs one more.
+template <typename T, int N> struct __attribute__((packed, aligned(sizeof(T)))) Q8Run {
+  T e[N];
+};
+
+// N (4 or 8) consecutive values of a row of C, of which the first n are there.
+template <typename T, int N> __device__ __forceinline__ void q8_store(T *p, const float (&v)[N], int64_t n)
 {
-  struct alignas(4 * sizeof(T)) Four { T e[4]; };
-  Four f;
+  constexpr int kPer = 16 / sizeof(T) < N ? 16 / sizeof(T) : N;
+  Q8Run<T, kPer> f[N / kPer];
 #pragma unroll
-  for (int i = 0; i < 4; i++) f.e[i] = q8_round<T>(v[i]);
-  if (aligned && n >= 4)
-    *(Four *)p = f;
-  else
-    for (int i = 0; i < 4; i++)
-      if (i < n) p[i] = f.e[i];
+  for (int i = 0; i < N; i++) f[i / kPer].e[i % kPer] = q8_round<T>(v[i]);
+  if (n >= N) {
+#pragma unroll
+    for (int i = 0; i < N / kPer; i++) *(Q8Run<T, kPer> *)(p + i * kPer) = f[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i++)
+      if (i < n) p[i] = f[i / kPer].e[i % kPer];
+  }
 }
 
 struct Q8Product {
@@ -206,7 +216,6 @@ struct Q8Product {
   int32_t blocks, sstride;
   void *out;
   int64_t os;                     // row stride of C
-  int32_t aligned;                // rows of C start at a multiple of 4 values' bytes
 };
 
 // Few rows (up to 16 a fragment): what bounds it is reading the draws once.  A wave takes 16 draws and every KS-th block
@@ -262,117 +271,316 @@ __global__ __launch_bounds__(1024) void q8_skinny_kernel(Q8Product a, int ks)
   }
   const int64_t j = j0 + g * 4;
   if (j >= a.draws) return;
-  const int n = a.draws - j < 4 ? (int)(a.draws - j) : 4;
 #pragma unroll
   for (int f = 0; f < RF; f++) {
     const int64_t i = i0 + f * 16 + r;
-    if (i < a.rows) q8_store4<T>((T *)a.out + i * a.os + j, acc[f], n, a.aligned);
+    const float v[4] = {acc[f][0], acc[f][1], acc[f][2], acc[f][3]};
+    if (i < a.rows) q8_store<T, 4>((T *)a.out + i * a.os + j, v, a.draws - j);
   }
 }
 
-// Many rows: a workgroup of four waves makes a 128 x 128 tile of C, 64 x 64 a wave.  A step of 128 columns of both sides
-// (16 KB each) comes straight from memory into LDS while the step before is multiplied.  A row's eight 16-byte pieces are
-// stored in an order that depends on the row, so that the eight lanes that read at a time touch all banks: row r of X has
-// piece c at place c ^ (r & 7).  Fragment f of a wave's draws takes the draws 16 (i / 4) + 4 f + i % 4 as its rows i, so
-// that a lane ends with 16 CONSECUTIVE values of a row of C over its four fragments; the order key of the draws' rows is
-// changed to fit.
-constexpr int kQ8Tile = 128;
-
-__device__ __forceinline__ int q8_draw_key(int r) { return (r & 3) | ((r >> 4) & 1) << 2; }
-
-template <typename T, bool WIDE>
-__global__ __launch_bounds__(kBlock) void q8_tile_kernel(Q8Product a, int tiles_n)
+// Narrow matrices (one or two blocks of columns: the samplers' own widths), many rows: C's bytes are what there is to
+// do.  A wave keeps 64 draws in registers and walks down the rows, 16 at a time, straight from memory into the
+// instruction's operand, the next 16 on their way; the four waves of a workgroup take neighbouring draws of the same rows.
+// Lane (r, g) holds bytes 16 g and 64 + 16 g of a block, so that four lanes read 64 consecutive bytes.  Fragment f of
+// the draws has draw 32 (f / 2) + 8 (i / 4) + 4 (f % 2) + i % 4 as its row i: a lane ends with two runs of eight values
+// of a row of C, four lanes with 64 consecutive bytes of a 16-bit type.
+template <typename T, bool WIDE, int BLOCKS>
+__global__ __launch_bounds__(kBlock) void q8_thin_kernel(Q8Product a, int groups_n, int walk)
 {
-  __shared__ __align__(1024) uint8_t lds[2][2][kQ8Tile * kQ8Block]; // [buffer][rows, draws]
-  const int tid = threadIdx.x, wave = tid / kWave, lane = tid % kWave, r = lane & 15, g = lane >> 4;
-  const int64_t i0 = (int64_t)(blockIdx.x / tiles_n) * kQ8Tile, j0 = (int64_t)(blockIdx.x % tiles_n) * kQ8Tile;
-  const int wi = (wave & 1) * 64, wj = (wave >> 1) * 64;
-  const int64_t xrows = a.rows - i0 < kQ8Tile ? a.rows - i0 : kQ8Tile, wrows = a.draws - j0 < kQ8Tile ? a.draws - j0 : kQ8Tile;
-  // rows past the end read as zeros: the descriptors end with the last row
-  const __amdgpu_buffer_rsrc_t xr = __builtin_amdgcn_make_buffer_rsrc((void *)(a.x + i0 * a.kp), 0, (int)(xrows * a.kp), 0x00020000);
-  const __amdgpu_buffer_rsrc_t wr = __builtin_amdgcn_make_buffer_rsrc((void *)(a.w + j0 * a.kp), 0, (int)(wrows * a.kp), 0x00020000);
-  const int lr = lane >> 3, lp = lane & 7;
-
-  auto fetch = [&](int buf, int b) {
-#pragma unroll
-    for (int q = 0; q < 4; q++) { // this wave's 32 rows of either side, 8 at a time
-      const int row = wave * 32 + q * 8 + lr;
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(xr, (__attribute__((address_space(3))) void *)(lds[buf][0] + (wave * 32 + q * 8) * kQ8Block), 16,
-                                               (int)(row * a.kp) + (lp ^ (row & 7)) * 16, b * kQ8Block, 0, 0);
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(wr, (__attribute__((address_space(3))) void *)(lds[buf][1] + (wave * 32 + q * 8) * kQ8Block), 16,
-                                               (int)(row * a.kp) + (lp ^ q8_draw_key(row)) * 16, b * kQ8Block, 0, 0);
-    }
-  };
-
-  // this lane's rows of the fragments; past the end any row's scale will do, its data are zeros
-  int xrow[4], wrow[4];
-  const uint8_t *xsp[4], *wsp[4];
-#pragma unroll
-  for (int f = 0; f < 4; f++) {
-    xrow[f] = wi + f * 16 + r;
-    wrow[f] = wj + (r >> 2) * 16 + f * 4 + (r & 3);
-    xsp[f] = a.xs + (i0 + (xrow[f] < xrows ? xrow[f] : xrows - 1)) * a.sstride;
-    wsp[f] = a.ws + (j0 + (wrow[f] < wrows ? wrow[f] : wrows - 1)) * a.sstride;
-  }
-  q8_f4 acc[4][4]; // [draws' fragment][rows' fragment]
-#pragma unroll
-  for (int f = 0; f < 4; f++)
-#pragma unroll
-    for (int h = 0; h < 4; h++) acc[f][h] = q8_f4{0.f, 0.f, 0.f, 0.f};
-
-  auto piece = [&](const uint8_t *base, int row, int key) {
-    const q8_i4 lo = *(const q8_i4 *)(base + row * kQ8Block + ((2 * g) ^ key) * 16);
-    const q8_i4 hi = *(const q8_i4 *)(base + row * kQ8Block + ((2 * g + 1) ^ key) * 16);
+#if defined(__HIP_DEVICE_COMPILE__)
+  const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave, r = lane & 15, g = lane >> 4;
+  const int64_t j0 = (int64_t)(blockIdx.x % groups_n) * 256 + wave * 64;
+  const int64_t from = (int64_t)(blockIdx.x / groups_n) * walk;
+  const int64_t to = from + walk < a.rows ? from + walk : a.rows;
+  if (j0 >= a.draws) return;
+  auto fragment = [&](const uint8_t *p) {
+    const q8_i4 lo = *(const q8_i4 *)(p + g * 16), hi = *(const q8_i4 *)(p + 64 + g * 16);
     return q8_i8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
   };
-
-  fetch(0, 0);
-  __syncthreads();
-  for (int b = 0; b < a.blocks; b++) {
-    const int buf = b & 1;
-    if (b + 1 < a.blocks) fetch(buf ^ 1, b + 1);
-    q8_i8 xv[4], wv[4];
-    uint32_t xc[4], wc[4];
+  q8_i8 wv[BLOCKS][4];
+  uint32_t ws[BLOCKS][4];
 #pragma unroll
-    for (int f = 0; f < 4; f++) {
-      xv[f] = piece(lds[buf][0], xrow[f], xrow[f] & 7);
-      wv[f] = piece(lds[buf][1], wrow[f], q8_draw_key(wrow[f]));
-      xc[f] = xsp[f][b];
-      wc[f] = wsp[f][b];
+  for (int f = 0; f < 4; f++) {
+    int64_t j = j0 + (f >> 1) * 32 + (r >> 2) * 8 + (f & 1) * 4 + (r & 3);
+    j = j < a.draws ? j : a.draws - 1;
+#pragma unroll
+    for (int b = 0; b < BLOCKS; b++) {
+      wv[b][f] = fragment(a.w + j * a.kp + b * kQ8Block);
+      ws[b][f] = a.ws[j * a.sstride + b];
     }
+  }
+  constexpr int kDown = BLOCKS == 1 ? 4 : 2; // fragments of rows under way
+  q8_i8 xn[kDown][BLOCKS];
+  uint32_t sn[kDown][BLOCKS];
+  auto fetch = [&](int64_t i0) {
+#pragma unroll
+    for (int d = 0; d < kDown; d++) {
+      const int64_t i = i0 + d * 16 + r < to ? i0 + d * 16 + r : to - 1;
+#pragma unroll
+      for (int b = 0; b < BLOCKS; b++) {
+        xn[d][b] = fragment(a.x + i * a.kp + b * kQ8Block);
+        sn[d][b] = a.xs[i * a.sstride + b];
+      }
+    }
+  };
+  // WHOLE: the wave's 64 draws are all there.  Rows past the end are the last one again and are stored as such, so that no
+  // branch lies between a fetch and its use: the wait for it would be one for the stores as well (one counter for both).
+  auto walk_down = [&](auto whole) {
+    fetch(from);
+    for (int64_t i0 = from; i0 < to; i0 += kDown * 16) {
+      q8_i8 xv[kDown][BLOCKS];
+      uint32_t xs[kDown][BLOCKS];
+#pragma unroll
+      for (int d = 0; d < kDown; d++)
+#pragma unroll
+        for (int b = 0; b < BLOCKS; b++) {
+          xv[d][b] = xn[d][b];
+          xs[d][b] = sn[d][b];
+        }
+      fetch(i0 + kDown * 16);
+#pragma unroll
+      for (int d = 0; d < kDown; d++) {
+        q8_f4 acc[4];
+#pragma unroll
+        for (int f = 0; f < 4; f++) acc[f] = q8_f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int b = 0; b < BLOCKS; b++) {
+          if (WIDE) {
+#pragma unroll
+            for (int s = 0; s < 4; s++) {
+              const q8_b8 xb = q8_widen(xv[d][b], s, q8_scale_value(xs[d][b]));
+#pragma unroll
+              for (int f = 0; f < 4; f++)
+                acc[f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(q8_widen(wv[b][f], s, q8_scale_value(ws[b][f])), xb, acc[f], 0, 0, 0);
+            }
+          } else {
+#pragma unroll
+            for (int f = 0; f < 4; f++)
+              acc[f] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wv[b][f], xv[d][b], acc[f], 0, 0, 0, (int)ws[b][f], 0, (int)xs[d][b]);
+          }
+        }
+        const int64_t i = i0 + d * 16 + r < to ? i0 + d * 16 + r : to - 1;
+#pragma unroll
+        for (int f = 0; f < 4; f += 2) {
+          const int64_t j = j0 + (f >> 1) * 32 + g * 8;
+          const float v[8] = {acc[f][0], acc[f][1], acc[f][2], acc[f][3], acc[f + 1][0], acc[f + 1][1], acc[f + 1][2], acc[f + 1][3]};
+          if (whole.value || j < a.draws) q8_store<T, 8>((T *)a.out + i * a.os + j, v, whole.value ? 8 : a.draws - j);
+        }
+      }
+    }
+  };
+  if (j0 + 64 <= a.draws)
+    walk_down(std::true_type{});
+  else
+    walk_down(std::false_type{});
+#endif
+}
+
+// Many rows, many columns: a workgroup of four waves makes a B x B tile of C (256, or 128 where that would leave CUs
+// without a tile), a quarter each.  A step of 128 columns of both sides comes straight from memory into LDS, a whole
+// line a row (64-byte pieces: 14 TB/s out of the L2s, lines: 24), into one of two buffers.  Registers hold half a step's
+// fragments twice, so that LDS is read for the next half while this one is multiplied, one read and one fetch to each
+// few matrix instructions.  In the middle of a step all of it has been read: one barrier, and its buffer is fetched into
+// again, a whole step before it is needed.
+// A ds_read_b128 serves lanes 0-3, 12-15, 20-23, 24-27 (and the like) together: q8_key orders the 16-byte pieces of a row
+// so that these 16 lanes touch 16 different places of 256 bytes (SQ_LDS_BANK_CONFLICT: 0).  Fragments are 32 x 32; a
+// draws' fragment has draw 16 (a / 2) + 8 g + 4 (a % 2) + e as its row 8 a + 4 g + e, which leaves a lane with runs of
+// eight values of a row of C.
+// Rows past the end: the last one again, never stored.
+__device__ __forceinline__ int q8_key(int row)
+{
+  const int q = row >> 2;
+  return ((row >> 1) & 1) | ((q ^ (q >> 1)) & 3) << 1;
+}
+
+// Tiles in the order in which workgroups start, which go to the eight dies in turn: a die has a run of tiles of its own,
+// four tile rows of C high, so that its L2 serves each line to several of its 32 CUs.
+__device__ __forceinline__ void q8_tile_of(int id, int tiles, int tiles_n, int *tm, int *tn)
+{
+  const int full = tiles / 8, rest = tiles % 8, die = id % 8;
+  const int t = die * full + (die < rest ? die : rest) + id / 8;
+  const int run = 4 * tiles_n, first = t / run * 4, tiles_m = tiles / tiles_n;
+  const int high = tiles_m - first < 4 ? tiles_m - first : 4, in = t % run;
+  *tm = first + in % high;
+  *tn = in / high;
+}
+
+template <typename T, bool WIDE, int B>
+__global__ __launch_bounds__(kBlock, B == 256 ? 1 : 2) void q8_tile_kernel(Q8Product a, int tiles_n, int tiles)
+{
+#if defined(__HIP_DEVICE_COMPILE__)
+  constexpr int F = B / 64;                  // fragments of 32 a wave has of either side
+  constexpr int kSide = B * kQ8Block, kFetch = B / 32; // bytes; kilobytes a wave fetches of either side
+  __shared__ __align__(1024) uint8_t lds[4 * kSide]; // [buffer][rows, draws][B][128]
+  const int tid = threadIdx.x, lane = tid % kWave, r = lane & 31, g = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+  int tm, tn;
+  q8_tile_of(blockIdx.x, tiles, tiles_n, &tm, &tn);
+  const int64_t i0 = (int64_t)tm * B, j0 = (int64_t)tn * B;
+  const int wi = (wave >> 1) * (B / 2), wj = (wave & 1) * (B / 2), kp = (int)a.kp;
+  const int xlast = (int)(a.rows - i0 < B ? a.rows - i0 : B) - 1, wlast = (int)(a.draws - j0 < B ? a.draws - j0 : B) - 1;
+  const __amdgpu_buffer_rsrc_t xr = __builtin_amdgcn_make_buffer_rsrc((void *)(a.x + i0 * a.kp), 0, (xlast + 1) * kp, 0x00020000);
+  const __amdgpu_buffer_rsrc_t wr = __builtin_amdgcn_make_buffer_rsrc((void *)(a.w + j0 * a.kp), 0, (wlast + 1) * kp, 0x00020000);
+  const uint8_t *xsp = a.xs + i0 * a.sstride, *wsp = a.ws + j0 * a.sstride;
+
+  int xvo[kFetch], wvo[kFetch]; // eight rows a fetch, eight lanes a row
+#pragma unroll
+  for (int q = 0; q < kFetch; q++) {
+    const int row = (wave * kFetch + q) * 8 + (lane >> 3), piece = ((lane & 7) ^ q8_key(row)) * 16;
+    xvo[q] = (row < xlast ? row : xlast) * kp + piece;
+    wvo[q] = (row < wlast ? row : wlast) * kp + piece;
+  }
+  auto fetch = [&](int b) {
+    uint8_t *to = lds + (b & 1) * 2 * kSide + wave * kFetch * 1024;
+#pragma unroll
+    for (int q = 0; q < kFetch; q++)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(xr, (__attribute__((address_space(3))) void *)(to + q * 1024), 16, xvo[q], b * kQ8Block, 0, 0);
+#pragma unroll
+    for (int q = 0; q < kFetch; q++)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(wr, (__attribute__((address_space(3))) void *)(to + kSide + q * 1024), 16, wvo[q], b * kQ8Block, 0, 0);
+  };
+
+  const int wl = (r >> 4) * 16 + ((r >> 2) & 1) * 8 + ((r >> 3) & 1) * 4 + (r & 3); // this lane's draw of a fragment
+  int xo[2][2], wo[2][2]; // [half of the step][16-byte piece]
+#pragma unroll
+  for (int h = 0; h < 2; h++)
+#pragma unroll
+    for (int q = 0; q < 2; q++) {
+      const int piece = h * 4 + 2 * g + q;
+      xo[h][q] = (wi + r) * kQ8Block + (piece ^ q8_key(r)) * 16;
+      wo[h][q] = kSide + (wj + wl) * kQ8Block + (piece ^ q8_key(wl)) * 16;
+    }
+  q8_i8 xv[2][F], wv[2][F];
+  auto read = [&](int h, int b) {
+    const uint8_t *base = lds + (b & 1) * 2 * kSide;
+#pragma unroll
+    for (int f = 0; f < F; f++) {
+      const q8_i4 lo = *(const q8_i4 *)(base + xo[h][0] + f * 32 * kQ8Block), hi = *(const q8_i4 *)(base + xo[h][1] + f * 32 * kQ8Block);
+      xv[h][f] = q8_i8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+    }
+#pragma unroll
+    for (int f = 0; f < F; f++) {
+      const q8_i4 lo = *(const q8_i4 *)(base + wo[h][0] + f * 32 * kQ8Block), hi = *(const q8_i4 *)(base + wo[h][1] + f * 32 * kQ8Block);
+      wv[h][f] = q8_i8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+    }
+  };
+
+  // Scales: one word has four blocks; the next word is loaded two steps before its first use.
+  int xso[F], wso[F];
+#pragma unroll
+  for (int f = 0; f < F; f++) {
+    const int i = wi + f * 32 + r, j = wj + f * 32 + wl;
+    xso[f] = (i < xlast ? i : xlast) * a.sstride;
+    wso[f] = (j < wlast ? j : wlast) * a.sstride;
+  }
+  uint32_t xs[F], ws[F], xsn[F], wsn[F];
+  auto scales = [&](int b) {
+#pragma unroll
+    for (int f = 0; f < F; f++) {
+      xsn[f] = *(const uint32_t *)(xsp + xso[f] + b);
+      wsn[f] = *(const uint32_t *)(wsp + wso[f] + b);
+    }
+  };
+
+  q8_f16 acc[F][F]; // [draws' fragment][rows' fragment]
+#pragma unroll
+  for (int f = 0; f < F; f++)
+#pragma unroll
+    for (int h = 0; h < F; h++)
+#pragma unroll
+      for (int e = 0; e < 16; e++) acc[f][h][e] = 0.f;
+  auto multiply = [&](int k) {
     if (WIDE) {
 #pragma unroll
       for (int s = 0; s < 4; s++) {
-        q8_b8 xb[4];
+        q8_b8 xb[F];
 #pragma unroll
-        for (int h = 0; h < 4; h++) xb[h] = q8_widen(xv[h], s, q8_scale_value(xc[h]));
+        for (int h = 0; h < F; h++) xb[h] = q8_widen(xv[k][h], s, q8_scale_value(xs[h] & 255u));
 #pragma unroll
-        for (int f = 0; f < 4; f++) {
-          const q8_b8 wb = q8_widen(wv[f], s, q8_scale_value(wc[f]));
+        for (int f = 0; f < F; f++) {
+          const q8_b8 wb = q8_widen(wv[k][f], s, q8_scale_value(ws[f] & 255u));
 #pragma unroll
-          for (int h = 0; h < 4; h++) acc[f][h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wb, xb[h], acc[f][h], 0, 0, 0);
+          for (int h = 0; h < F; h++) acc[f][h] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wb, xb[h], acc[f][h], 0, 0, 0);
         }
       }
     } else {
 #pragma unroll
-      for (int f = 0; f < 4; f++)
+      for (int f = 0; f < F; f++)
 #pragma unroll
-        for (int h = 0; h < 4; h++)
-          acc[f][h] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wv[f], xv[h], acc[f][h], 0, 0, 0, (int)wc[f], 0, (int)xc[h]);
+        for (int h = 0; h < F; h++)
+          acc[f][h] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wv[k][f], xv[k][h], acc[f][h], 0, 0, 0, (int)ws[f], 0, (int)xs[h]);
     }
-    __syncthreads(); // the next step has arrived (the barrier waits for this wave's loads), this one has been read
-  }
+  };
+  // For the scheduler: of a half's 4 F reads (and 2 kFetch fetches) an equal share before each of F F groups of products
+  constexpr int kGroups = F * F, kReads = 4 * F / kGroups, kFetches = 2 * kFetch / kGroups, kProducts = WIDE ? 4 : 1;
+
+  scales(0);
+  fetch(0);
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  if (a.blocks > 1) fetch(1);
+  read(0, 0);
+  auto step = [&](int b, auto more) {
+    if ((b & 3) == 0) {
+#pragma unroll
+      for (int f = 0; f < F; f++) {
+        xs[f] = xsn[f];
+        ws[f] = wsn[f];
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    read(1, b);
+    multiply(0);
+#pragma unroll
+    for (int i = 0; i < kGroups; i++) {
+      __builtin_amdgcn_sched_group_barrier(0x100, kReads, 0);
+      __builtin_amdgcn_sched_group_barrier(0x8, kProducts, 0);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    // this wave has read all of the step, and has its part of the next; behind the barrier, all waves
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+    if (more.value) {
+      if ((b & 3) == 2) scales(b + 2);
+      fetch(b + 2);
+    }
+    read(0, b + 1); // past the last step: what lies there, unused
+    multiply(1);
+#pragma unroll
+    for (int i = 0; i < kGroups; i++) {
+      __builtin_amdgcn_sched_group_barrier(0x100, kReads, 0);
+      if (more.value) __builtin_amdgcn_sched_group_barrier(0x20, kFetches, 0);
+      __builtin_amdgcn_sched_group_barrier(0x8, kProducts, 0);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int f = 0; f < F; f++) {
+      xs[f] >>= 8;
+      ws[f] >>= 8;
+    }
+  };
+  int b = 0;
+  for (; b < a.blocks - 2; b++) step(b, std::true_type{});
+  for (; b < a.blocks; b++) step(b, std::false_type{});
 
 #pragma unroll
-  for (int h = 0; h < 4; h++) {
-    const int64_t i = i0 + xrow[h];
+  for (int h = 0; h < F; h++) {
+    const int64_t i = i0 + wi + h * 32 + r;
     if (i >= a.rows) continue;
 #pragma unroll
-    for (int f = 0; f < 4; f++) {
-      const int64_t j = j0 + wj + g * 16 + f * 4;
-      if (j < a.draws) q8_store4<T>((T *)a.out + i * a.os + j, acc[f][h], a.draws - j < 4 ? (int)(a.draws - j) : 4, a.aligned);
-    }
+    for (int f = 0; f < F; f++)
+#pragma unroll
+      for (int q = 0; q < 2; q++) {
+        const int64_t j = j0 + wj + f * 32 + q * 16 + g * 8;
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) v[e] = acc[f][h][q * 8 + e];
+        if (j < a.draws) q8_store<T, 8>((T *)a.out + i * a.os + j, v, a.draws - j);
+      }
   }
+#endif
 }
 
 } // namespace mhlik
