@@ -77,13 +77,8 @@ int quantize_launch(const T *x, int64_t rows, int64_t cols, int64_t rs, int64_t 
   } else {
     const int64_t units = rows * blocks, groups = (units * 16 + kBlock - 1) / kBlock;
     if (groups > INT32_MAX) return fail_no_ctx(MHLIK_EINVAL, "too many blocks (%lld)", (long long)units);
-    const bool vec = cs == 1 && aligned16(x) && (rows == 1 || rs * (int64_t)sizeof(T) % 16 == 0);
-    if (vec)
-      hipLaunchKernelGGL((q8_rows_kernel<T, true>), dim3((unsigned)groups), dim3(kBlock), 0, stream, x, units, cols, rs, cs,
-                         (uint32_t)blocks, (uint32_t)sstride, data, scale);
-    else
-      hipLaunchKernelGGL((q8_rows_kernel<T, false>), dim3((unsigned)groups), dim3(kBlock), 0, stream, x, units, cols, rs, cs,
-                         (uint32_t)blocks, (uint32_t)sstride, data, scale);
+    hipLaunchKernelGGL(q8_rows_kernel<T>, dim3((unsigned)groups), dim3(kBlock), 0, stream, Q8Values{x, rs, cs, 0}, units, cols,
+                       (uint32_t)blocks, (uint32_t)sstride, data, scale);
   }
   PCHK(hipGetLastError());
   return MHLIK_OK;
@@ -116,7 +111,11 @@ int check_values(const char *what, const void *x, int32_t type, int64_t rows, in
   return MHLIK_OK;
 }
 
-template <typename T> int product_launch(const Q8Product &a, hipStream_t stream)
+// Rows that the few-rows kernel quantizes by itself.
+bool few_rows(int64_t rows, int64_t cols) { return rows <= 64 && rows * q8_blocks(cols) * kQ8Block <= kQ8FewBytes; }
+
+// values.type != 0: the rows are those (few_rows says that they are few enough), not a.x
+template <typename T> int product_launch(const Q8Product &a, const Q8Values &values, hipStream_t stream)
 {
   constexpr bool kWide = sizeof(T) == 4;
   // Up to 64 rows a wave keeps all of them beside 16 draws, so that the draws are read once for all rows; more rows go
@@ -124,18 +123,24 @@ template <typename T> int product_launch(const Q8Product &a, hipStream_t stream)
   if (a.rows <= 64) {
     const int rf = a.rows <= 16 ? 1 : a.rows <= 32 ? 2 : 4;
     const int64_t groups16 = (a.draws + 15) / 16;
-    int ks = 1; // waves that share 16 draws: until the chip's 1024 SIMDs have two each, or a wave's part is two steps
-    while (ks < 16 && groups16 * ks < 2048 && a.blocks >= 4 * ks) ks *= 2;
+    int ks = 1; // waves that share 16 draws: until the chip's 1024 SIMDs have four each, or a wave's part is two steps
+    while (ks < 8 && groups16 * ks < 4096 && a.blocks >= 4 * ks) ks *= 2;
     const int waves = ks < 4 ? 4 : ks;
     const int64_t groups = (groups16 + waves / ks - 1) / (waves / ks);
     if (groups > INT32_MAX) return fail_no_ctx(MHLIK_EINVAL, "too many draws (%lld)", (long long)a.draws);
     const dim3 grid((unsigned)groups), block(waves * kWave);
-    if (rf == 1)
-      hipLaunchKernelGGL((q8_skinny_kernel<T, 1>), grid, block, 0, stream, a, ks);
+    if (values.type && rf == 1)
+      hipLaunchKernelGGL((q8_skinny_kernel<T, 1, true>), grid, block, 0, stream, a, values, ks);
+    else if (values.type && rf == 2)
+      hipLaunchKernelGGL((q8_skinny_kernel<T, 2, true>), grid, block, 0, stream, a, values, ks);
+    else if (values.type)
+      hipLaunchKernelGGL((q8_skinny_kernel<T, 4, true>), grid, block, 0, stream, a, values, ks);
+    else if (rf == 1)
+      hipLaunchKernelGGL((q8_skinny_kernel<T, 1, false>), grid, block, 0, stream, a, values, ks);
     else if (rf == 2)
-      hipLaunchKernelGGL((q8_skinny_kernel<T, 2>), grid, block, 0, stream, a, ks);
+      hipLaunchKernelGGL((q8_skinny_kernel<T, 2, false>), grid, block, 0, stream, a, values, ks);
     else
-      hipLaunchKernelGGL((q8_skinny_kernel<T, 4>), grid, block, 0, stream, a, ks);
+      hipLaunchKernelGGL((q8_skinny_kernel<T, 4, false>), grid, block, 0, stream, a, values, ks);
   } else if (a.blocks <= 2) {
     const int64_t gn = (a.draws + 255) / 256;
     int64_t walk = 512; // rows a workgroup walks down: fewer where the chip would not be full
@@ -275,7 +280,7 @@ int mhlik_q8_product_workspace(int64_t rows, int64_t cols, size_t *bytes)
 {
   if (!bytes) return fail_no_ctx(MHLIK_EINVAL, "bytes must not be NULL");
   if (int rc = check_shape(rows, cols)) return rc;
-  *bytes = (size_t)rows * (size_t)(q8_blocks(cols) * kQ8Block + q8_scale_stride(cols));
+  *bytes = few_rows(rows, cols) ? 0 : (size_t)rows * (size_t)(q8_blocks(cols) * kQ8Block + q8_scale_stride(cols));
   return MHLIK_OK;
 }
 
@@ -303,15 +308,20 @@ int mhlik_q8_product(const mhlik_q8_operands *p, int32_t device, void *stream)
   a.rows = p->rows;
   a.draws = p->draws;
   a.blocks = (int32_t)q8_blocks(p->cols);
+  a.cols = p->cols;
   a.kp = (int64_t)a.blocks * kQ8Block;
   a.sstride = (int32_t)q8_scale_stride(p->cols);
   a.w = p->w_data;
   a.ws = p->w_scale;
   a.out = p->out;
   a.os = p->out_stride;
+  Q8Values values = {nullptr, 0, 0, MHLIK_T_Q8};
   if (ready) {
     a.x = (const uint8_t *)p->x;
     a.xs = p->x_scale;
+  } else if (few_rows(p->rows, p->cols)) {
+    values = Q8Values{p->x, p->x_row_stride, p->x_col_stride, p->x_type};
+    a.x = a.xs = nullptr;
   } else {
     const size_t need = (size_t)p->rows * (size_t)(a.kp + a.sstride);
     if (!p->workspace || !aligned16(p->workspace) || p->workspace_bytes < need)
@@ -322,9 +332,9 @@ int mhlik_q8_product(const mhlik_q8_operands *p, int32_t device, void *stream)
     a.xs = scale;
   }
   switch (p->out_type) {
-  case MHLIK_T_F32: return product_launch<float>(a, (hipStream_t)stream);
-  case MHLIK_T_BF16: return product_launch<__bf16>(a, (hipStream_t)stream);
-  default: return product_launch<_Float16>(a, (hipStream_t)stream);
+  case MHLIK_T_F32: return product_launch<float>(a, values, (hipStream_t)stream);
+  case MHLIK_T_BF16: return product_launch<__bf16>(a, values, (hipStream_t)stream);
+  default: return product_launch<_Float16>(a, values, (hipStream_t)stream);
   }
 }
 

@@ -38,10 +38,9 @@ template <typename T> __device__ __forceinline__ float q8_load(T v) { return (fl
 template <> __device__ __forceinline__ float q8_load<double>(double v)
 {
   const float f = (float)v;
-  if ((double)f == v || v != v || fabs(v) == HUGE_VAL) return f;
   uint32_t b = __float_as_uint(f);
-  if (fabs((double)f) > fabs(v)) b--; // toward zero
-  return __uint_as_float(b | 1u);
+  b -= fabs((double)f) > fabs(v); // toward zero
+  return (double)f < v || (double)f > v ? __uint_as_float(b | 1u) : f;
 }
 
 __device__ __forceinline__ float q8_finite_abs(float v)
@@ -71,47 +70,75 @@ __device__ __forceinline__ uint32_t q8_pack4(float a, float b, float c, float d)
   return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true);
 }
 
+// Values that go to or come from any address of their type in one access: gfx950 takes unaligned ones, an access that
+// spans two lines costs one more.
+template <typename T, int N> struct __attribute__((packed, aligned(sizeof(T)))) Q8Run {
+  T e[N];
+};
+
+// Values of a matrix whose type the kernel learns at run time (the same numbers as MHLIK_T_*).
+struct Q8Values {
+  const void *x;
+  int64_t rs, cs;
+  int32_t type; // 1 double, 2 float, 3 bfloat16, 4 half; 0: there are none
+};
+
+// Eight values of a row, from column c0; 0 from column n on.
+template <typename T> __device__ __forceinline__ void q8_eight(const Q8Values &x, int64_t row, int64_t c0, int64_t n, float (&v)[kQ8Lane])
+{
+  const T *p = (const T *)x.x + row * x.rs + c0 * x.cs;
+  if (x.cs == 1 && c0 + kQ8Lane <= n) {
+    const Q8Run<T, kQ8Lane> q = *(const Q8Run<T, kQ8Lane> *)p;
+#pragma unroll
+    for (int i = 0; i < kQ8Lane; i++) v[i] = q8_load<T>(q.e[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kQ8Lane; i++) v[i] = c0 + i < n ? q8_load<T>(p[i * x.cs]) : 0.f;
+  }
+}
+
+__device__ __forceinline__ void q8_eight(const Q8Values &x, int64_t row, int64_t c0, int64_t n, float (&v)[kQ8Lane])
+{
+  switch (x.type) {
+  case 1: return q8_eight<double>(x, row, c0, n, v);
+  case 2: return q8_eight<float>(x, row, c0, n, v);
+  case 3: return q8_eight<__bf16>(x, row, c0, n, v);
+  default: return q8_eight<_Float16>(x, row, c0, n, v);
+  }
+}
+
+// A block's share of one of 16 lanes: its eight values as bytes, and k.
+__device__ __forceinline__ uint2 q8_pack_block(const float (&v)[kQ8Lane], int *k)
+{
+  float top = 0.f;
+#pragma unroll
+  for (int i = 0; i < kQ8Lane; i++) top = fmaxf(top, q8_finite_abs(v[i]));
+#pragma unroll
+  for (int m = 1; m < 16; m <<= 1) top = fmaxf(top, __shfl_xor(top, m, 16));
+  *k = q8_exponent(top);
+  const float inv = __uint_as_float((uint32_t)(127 - *k) << 23);
+  uint2 out;
+  out.x = q8_pack4(q8_scaled(v[0], inv), q8_scaled(v[1], inv), q8_scaled(v[2], inv), q8_scaled(v[3], inv));
+  out.y = q8_pack4(q8_scaled(v[4], inv), q8_scaled(v[5], inv), q8_scaled(v[6], inv), q8_scaled(v[7], inv));
+  return out;
+}
+
 // Rows: 16 lanes take one block, 8 consecutive columns a lane (16 bytes of a 16-bit type in one load, 64 of a double in
-// four), the block's largest magnitude goes round the 16 lanes in four exchanges.  VEC: every lane's columns start at a
-// multiple of 16 bytes and the last block is whole, or else its columns are loaded one by one.
+// four), the block's largest magnitude goes round the 16 lanes in four exchanges.
 // Memory bound: cols sizeof(T) bytes read, cols written, nothing kept.
-template <typename T, bool VEC>
-__global__ __launch_bounds__(kBlock) void q8_rows_kernel(const T *__restrict__ x, int64_t units, int64_t cols, int64_t rs,
-                                                         int64_t cs, uint32_t blocks, uint32_t sstride,
+template <typename T>
+__global__ __launch_bounds__(kBlock) void q8_rows_kernel(Q8Values x, int64_t units, int64_t cols, uint32_t blocks, uint32_t sstride,
                                                          uint8_t *__restrict__ data, uint8_t *__restrict__ scale)
 {
   const int64_t unit = ((int64_t)blockIdx.x * kBlock + threadIdx.x) / 16;
   const int l = threadIdx.x & 15;
   if (unit >= units) return; // whole groups of 16 lanes
   const int64_t row = blocks == 1 ? unit : unit < (int64_t)1 << 32 ? (int64_t)((uint32_t)unit / blocks) : unit / blocks;
-  const int64_t blk = unit - row * blocks;
-  const int64_t c0 = blk * kQ8Block + l * kQ8Lane;
+  const int64_t blk = unit - row * blocks, c0 = blk * kQ8Block + l * kQ8Lane;
   float v[kQ8Lane];
-  const T *p = x + row * rs + c0 * (VEC ? 1 : cs);
-  if (VEC && c0 + kQ8Lane <= cols) {
-    struct alignas(16) Pack { T e[16 / sizeof(T)]; };
-    constexpr int kPer = 16 / sizeof(T);
-#pragma unroll
-    for (int i = 0; i < kQ8Lane / kPer; i++) {
-      const Pack q = ((const Pack *)p)[i];
-#pragma unroll
-      for (int j = 0; j < kPer; j++) v[i * kPer + j] = q8_load<T>(q.e[j]);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < kQ8Lane; i++) v[i] = c0 + i < cols ? q8_load<T>(p[i * (VEC ? 1 : cs)]) : 0.f;
-  }
-  float top = 0.f;
-#pragma unroll
-  for (int i = 0; i < kQ8Lane; i++) top = fmaxf(top, q8_finite_abs(v[i]));
-#pragma unroll
-  for (int m = 1; m < 16; m <<= 1) top = fmaxf(top, __shfl_xor(top, m, 16));
-  const int k = q8_exponent(top);
-  const float inv = __uint_as_float((uint32_t)(127 - k) << 23);
-  uint2 out;
-  out.x = q8_pack4(q8_scaled(v[0], inv), q8_scaled(v[1], inv), q8_scaled(v[2], inv), q8_scaled(v[3], inv));
-  out.y = q8_pack4(q8_scaled(v[4], inv), q8_scaled(v[5], inv), q8_scaled(v[6], inv), q8_scaled(v[7], inv));
-  *(uint2 *)(data + row * blocks * kQ8Block + c0) = out;
+  q8_eight<T>(x, row, c0, cols, v);
+  int k;
+  *(uint2 *)(data + row * blocks * kQ8Block + c0) = q8_pack_block(v, &k);
   if (l == 0) {
     uint8_t *s = scale + row * sstride + blk;
     *s = (uint8_t)(k + 127);
@@ -129,16 +156,26 @@ __global__ __launch_bounds__(kBlock) void q8_columns_kernel(const T *__restrict_
 {
   const int64_t row = (int64_t)blockIdx.x * kBlock + threadIdx.x;
   if (row >= rows) return;
+  constexpr int kAtOnce = 16; // columns whose loads are under way together
   const uint32_t blk = blockIdx.y;
   const int64_t c0 = (int64_t)blk * kQ8Block;
   const int n = cols - c0 < kQ8Block ? (int)(cols - c0) : kQ8Block;
   const T *p = x + row + c0 * cs;
-  float v[kQ8Block];
-  float top = 0.f;
+  float v[kQ8Block], top = 0.f;
 #pragma unroll
-  for (int i = 0; i < kQ8Block; i++) {
-    v[i] = i < n ? q8_load<T>(p[i * cs]) : 0.f;
-    top = fmaxf(top, q8_finite_abs(v[i]));
+  for (int i = 0; i < kQ8Block; i += kAtOnce) {
+    if (i + kAtOnce <= n) {
+      T t[kAtOnce];
+#pragma unroll
+      for (int q = 0; q < kAtOnce; q++) t[q] = p[(i + q) * cs];
+#pragma unroll
+      for (int q = 0; q < kAtOnce; q++) v[i + q] = q8_load<T>(t[q]);
+    } else {
+#pragma unroll
+      for (int q = 0; q < kAtOnce; q++) v[i + q] = i + q < n ? q8_load<T>(p[(i + q) * cs]) : 0.f;
+    }
+#pragma unroll
+    for (int q = 0; q < kAtOnce; q++) top = fmaxf(top, q8_finite_abs(v[i + q]));
   }
   const int k = q8_exponent(top);
   const float inv = __uint_as_float((uint32_t)(127 - k) << 23);
@@ -186,12 +223,6 @@ __device__ __forceinline__ q8_b8 q8_widen(q8_i8 v, int s, float scale)
 
 template <typename T> __device__ __forceinline__ T q8_round(float v) { return (T)v; }
 
-// Values that go to or come from any address of their type in one access: gfx950 takes unaligned ones, an access that
-// spans two lines costs one more.
-template <typename T, int N> struct __attribute__((packed, aligned(sizeof(T)))) Q8Run {
-  T e[N];
-};
-
 // N (4 or 8) consecutive values of a row of C, of which the first n are there.
 template <typename T, int N> __device__ __forceinline__ void q8_store(T *p, const float (&v)[N], int64_t n)
 {
@@ -212,68 +243,112 @@ template <typename T, int N> __device__ __forceinline__ void q8_store(T *p, cons
 struct Q8Product {
   const uint8_t *x, *xs, *w, *ws; // data and scales of rows and draws
   int64_t rows, draws;
+  int64_t cols;
   int64_t kp;                     // padded columns: bytes per row
   int32_t blocks, sstride;
   void *out;
   int64_t os;                     // row stride of C
 };
 
-// Few rows (up to 16 a fragment): what bounds it is reading the draws once.  A wave takes 16 draws and every KS-th block
-// of 128 columns; its lanes load 32 consecutive bytes of a draw straight into the instruction's operand, 4 lanes a block.
-// The KS waves of a 16-draw group add up through LDS in wave order.  The draws are the instruction's rows, so that a
-// lane ends with four consecutive values of one row of C.
-template <typename T, int RF>
-__global__ __launch_bounds__(1024) void q8_skinny_kernel(Q8Product a, int ks)
+// Few rows (up to 16 a fragment, RF fragments): what bounds it is reading the draws once.  A wave takes 16 draws and every
+// ks-th block of 128 columns; its lanes load 32 consecutive bytes of a draw straight into the instruction's operand, 4
+// lanes a block, four blocks ahead of the four being multiplied.  The ks waves of a 16-draw group add up through LDS in
+// wave order.  The draws are the instruction's rows, so that a lane ends with four consecutive values of one row of C.
+// FROM_VALUES: the rows come as values; each workgroup quantizes all of them into LDS (they are few: up to 16 KB) while
+// its first draws are on their way, which saves a kernel and its start.
+constexpr int kQ8FewBytes = 16384;
+
+template <typename T, int RF, bool FROM_VALUES>
+__global__ __launch_bounds__(512) void q8_skinny_kernel(Q8Product a, Q8Values values, int ks)
 {
-  __shared__ q8_f4 part[16][RF][kWave];
-  const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave, r = lane & 15, g = lane >> 4;
+  __shared__ __align__(16) q8_f4 part[RF == 1 ? 16 : 8 * RF][kWave]; // the rows' bytes and scales first, then the waves' sums
+  static_assert(sizeof(part) >= kQ8FewBytes, "room for the rows");
+  __shared__ uint8_t codes[FROM_VALUES ? kQ8FewBytes / kQ8Block : 1];
+  const int tid = threadIdx.x, wave = tid / kWave, lane = tid % kWave, r = lane & 15, g = lane >> 4;
   const int kw = wave % ks, nw = blockDim.x / kWave;
   const int64_t j0 = ((int64_t)blockIdx.x * (nw / ks) + wave / ks) * 16;
   const int64_t jr = j0 + r < a.draws ? j0 + r : a.draws - 1; // past the end: the last draw again, not stored
   const uint8_t *w = a.w + jr * a.kp + g * 32, *ws = a.ws + jr * a.sstride;
-  const int64_t i0 = (int64_t)blockIdx.y * 16 * RF;
+  constexpr int kAhead = 4;
+  q8_i8 wn[kAhead];
+  uint32_t sn[kAhead];
+  auto fetch = [&](int b0) {
+#pragma unroll
+    for (int q = 0; q < kAhead; q++) {
+      const int b = b0 + q * ks < a.blocks ? b0 + q * ks : a.blocks - 1;
+      wn[q] = *(const q8_i8 *)(w + (int64_t)b * kQ8Block);
+      sn[q] = ws[b];
+    }
+  };
+  fetch(kw);
+  uint8_t *bytes = (uint8_t *)part;
+  if (FROM_VALUES) {
+    const int l = tid & 15, units = (int)a.rows * a.blocks;
+    for (int unit = tid / 16; unit < units; unit += blockDim.x / 16) {
+      const int row = unit / a.blocks;
+      const int64_t c0 = (int64_t)(unit - row * a.blocks) * kQ8Block + l * kQ8Lane;
+      float v[kQ8Lane];
+      q8_eight(values, row, c0, a.cols, v);
+      int k;
+      *(uint2 *)(bytes + unit * kQ8Block + l * kQ8Lane) = q8_pack_block(v, &k);
+      if (l == 0) codes[unit] = (uint8_t)(k + 127);
+    }
+    __syncthreads();
+  }
   const uint8_t *x[RF], *xs[RF];
 #pragma unroll
   for (int f = 0; f < RF; f++) {
-    const int64_t ir = i0 + f * 16 + r < a.rows ? i0 + f * 16 + r : a.rows - 1;
-    x[f] = a.x + ir * a.kp + g * 32;
-    xs[f] = a.xs + ir * a.sstride;
+    const int64_t ir = f * 16 + r < a.rows ? f * 16 + r : a.rows - 1;
+    x[f] = (FROM_VALUES ? bytes : a.x) + ir * a.kp + g * 32;
+    xs[f] = FROM_VALUES ? codes + ir * a.blocks : a.xs + ir * a.sstride;
   }
   q8_f4 acc[RF];
 #pragma unroll
   for (int f = 0; f < RF; f++) acc[f] = q8_f4{0.f, 0.f, 0.f, 0.f};
-  for (int b = kw; b < a.blocks; b += ks) {
-    const q8_i8 wv = *(const q8_i8 *)(w + (int64_t)b * kQ8Block);
-    const float wsv = q8_scale_value(ws[b]);
-    q8_i8 xv[RF];
-    float xsv[RF];
+  for (int b0 = kw; b0 < a.blocks; b0 += kAhead * ks) {
+    q8_i8 wv[kAhead];
+    uint32_t sv[kAhead];
 #pragma unroll
-    for (int f = 0; f < RF; f++) {
-      xv[f] = *(const q8_i8 *)(x[f] + (int64_t)b * kQ8Block);
-      xsv[f] = q8_scale_value(xs[f][b]);
+    for (int q = 0; q < kAhead; q++) {
+      wv[q] = wn[q];
+      sv[q] = sn[q];
     }
+    if (b0 + kAhead * ks < a.blocks) fetch(b0 + kAhead * ks);
 #pragma unroll
-    for (int s = 0; s < 4; s++) {
-      const q8_b8 wb = q8_widen(wv, s, wsv);
+    for (int q = 0; q < kAhead; q++) {
+      const int b = b0 + q * ks;
+      if (b >= a.blocks) break;
+      q8_i8 xv[RF];
+      float xsv[RF];
 #pragma unroll
-      for (int f = 0; f < RF; f++)
-        acc[f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wb, q8_widen(xv[f], s, xsv[f]), acc[f], 0, 0, 0);
+      for (int f = 0; f < RF; f++) {
+        xv[f] = *(const q8_i8 *)(x[f] + b * kQ8Block);
+        xsv[f] = q8_scale_value(xs[f][b]);
+      }
+#pragma unroll
+      for (int s = 0; s < 4; s++) {
+        const q8_b8 wb = q8_widen(wv[q], s, q8_scale_value(sv[q]));
+#pragma unroll
+        for (int f = 0; f < RF; f++)
+          acc[f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wb, q8_widen(xv[f], s, xsv[f]), acc[f], 0, 0, 0);
+      }
     }
   }
   if (ks > 1) {
+    if (FROM_VALUES) __syncthreads(); // the rows have been read
 #pragma unroll
-    for (int f = 0; f < RF; f++) part[wave][f][lane] = acc[f];
+    for (int f = 0; f < RF; f++) part[wave * RF + f][lane] = acc[f];
     __syncthreads();
     if (kw) return;
     for (int q = 1; q < ks; q++)
 #pragma unroll
-      for (int f = 0; f < RF; f++) acc[f] += part[wave + q][f][lane];
+      for (int f = 0; f < RF; f++) acc[f] += part[(wave + q) * RF + f][lane];
   }
   const int64_t j = j0 + g * 4;
   if (j >= a.draws) return;
 #pragma unroll
   for (int f = 0; f < RF; f++) {
-    const int64_t i = i0 + f * 16 + r;
+    const int64_t i = f * 16 + r;
     const float v[4] = {acc[f][0], acc[f][1], acc[f][2], acc[f][3]};
     if (i < a.rows) q8_store<T, 4>((T *)a.out + i * a.os + j, v, a.draws - j);
   }

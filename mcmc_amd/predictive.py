@@ -6,6 +6,7 @@ sampler has kept.  Work is queued on the tensors' GPU, on torch's current stream
 it has gradients: inputs that require them are refused while gradients are recorded.
 """
 import ctypes as C
+import functools
 
 import torch
 
@@ -16,6 +17,10 @@ BLOCK = 128
 _TYPES = {torch.float64: L.T_F64, torch.float32: L.T_F32, torch.bfloat16: L.T_BF16, torch.float16: L.T_F16}
 _OUT = {torch.float32: L.T_F32, torch.bfloat16: L.T_BF16, torch.float16: L.T_F16}
 _U = {torch.float64: L.T_F64, torch.float32: L.T_F32}
+_E4M3 = {torch.float8_e4m3fn: L.T_Q8}
+_CODE = {torch.uint8: None}
+
+_grad = torch.is_grad_enabled
 
 
 def _chk(rc):
@@ -29,68 +34,74 @@ def _need(ok, text, *args):
 
 
 def _given(name, t, dims, types):
+    """The tensor's device, after the checks that every argument has to pass."""
+    if isinstance(t, torch.Tensor) and t.is_cuda and t.dim() == dims and t.dtype in types and not (t.requires_grad and _grad()):
+        return t.device
     _need(isinstance(t, torch.Tensor), "%s must be a tensor", name)
     _need(t.is_cuda, "%s must be on a GPU: there is no CPU path", name)
     _need(t.dim() == dims, "%s must have %d dimension(s), not %d", name, dims, t.dim())
     _need(t.dtype in types, "%s has type %s; wanted: %s", name, t.dtype, ", ".join(str(x) for x in types))
-    _need(not (t.requires_grad and torch.is_grad_enabled()), "%s requires a gradient, and there is none: detach it", name)
+    raise ValueError("%s requires a gradient, and there is none: detach it" % name)
 
 
-def _same(name, t, device):
-    _need(t.device == device, "%s is on %s, the rest on %s", name, t.device, device)
+def _same(name, device, wanted):
+    if device != wanted:
+        raise ValueError("%s is on %s, the rest on %s" % (name, device, wanted))
 
 
-def _stream(device):
-    return torch.cuda.current_stream(device).cuda_stream
+# The current stream's handle without building a Stream object (a call costs 2 us otherwise); both say the same.
+_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 class Block8:
     """Rows of `cols` values in 8 bits: `data` float8_e4m3fn [rows, 128 ceil(cols / 128)], columns past the last 0, and
     `scale` uint8 [rows, 4 ceil(cols / 512)]: the 128 columns of block b stand for data * 2^(scale[:, b] - 127)."""
 
-    __slots__ = ("data", "scale", "cols")
+    __slots__ = ("data", "scale", "cols", "rows", "device")
 
     def __init__(self, data, scale, cols):
-        _given("data", data, 2, (torch.float8_e4m3fn,))
-        _given("scale", scale, 2, (torch.uint8,))
-        _same("scale", scale, data.device)
+        device = _given("data", data, 2, _E4M3)
+        _same("scale", _given("scale", scale, 2, _CODE), device)
+        rows, wide = data.shape
         blocks = -(-cols // BLOCK)
         _need(cols >= 1, "cols must be at least 1, not %d", cols)
-        _need(data.shape[1] == blocks * BLOCK, "data has %d columns; %d are %d in blocks of %d", data.shape[1], cols, blocks * BLOCK, BLOCK)
-        _need(tuple(scale.shape) == (data.shape[0], 4 * -(-blocks // 4)), "scale has shape %s; wanted %s", tuple(scale.shape),
-              (data.shape[0], 4 * -(-blocks // 4)))
+        _need(wide == blocks * BLOCK, "data has %d columns; %d are %d in blocks of %d", wide, cols, blocks * BLOCK, BLOCK)
+        if scale.shape != (rows, (blocks + 3) // 4 * 4):
+            raise ValueError("scale has shape %s; wanted %s" % (tuple(scale.shape), (rows, (blocks + 3) // 4 * 4)))
         _need(data.is_contiguous() and scale.is_contiguous(), "data and scale must be contiguous")
         _need(data.data_ptr() % 16 == 0, "data must start at a multiple of 16 bytes")
-        self.data, self.scale, self.cols = data, scale, int(cols)
-
-    @property
-    def rows(self):
-        return self.data.shape[0]
+        self.data, self.scale, self.cols, self.rows, self.device = data, scale, int(cols), rows, device
 
     def dequantize(self):
         """The values the rows stand for, as float32 [rows, cols]."""
         blocks = self.data.shape[1] // BLOCK
-        step = torch.ldexp(torch.ones((), device=self.data.device), self.scale[:, :blocks].int() - 127)
+        step = torch.ldexp(torch.ones((), device=self.device), self.scale[:, :blocks].int() - 127)
         return (self.data.float().view(-1, blocks, BLOCK) * step[:, :, None]).view(self.data.shape)[:, : self.cols]
-
-
-def _empty8(rows, cols, device):
-    blocks = -(-cols // BLOCK)
-    return (torch.empty(rows, blocks * BLOCK, dtype=torch.float8_e4m3fn, device=device),
-            torch.empty(rows, 4 * -(-blocks // 4), dtype=torch.uint8, device=device))
 
 
 def quantize(x):
     """Rows x [rows, cols] (float64, float32, bfloat16 or float16; any strides) as Block8: each value is rounded once, to
     the nearest e4m3 value on the scale of its block.  What is not finite, or above 448 * 2^119, becomes NaN."""
-    _given("x", x, 2, _TYPES)
+    device = _given("x", x, 2, _TYPES)
     rows, cols = x.shape
     _need(cols >= 1, "x must have at least one column")
-    data, scale = _empty8(rows, cols, x.device)
+    blocks = -(-cols // BLOCK)
+    q = Block8.__new__(Block8)  # as its constructor would have it
+    q.data = torch.empty((rows, blocks * BLOCK), dtype=torch.float8_e4m3fn, device=device)
+    q.scale = torch.empty((rows, (blocks + 3) // 4 * 4), dtype=torch.uint8, device=device)
+    q.cols, q.rows, q.device = cols, rows, device
     rs, cs = x.stride()
-    _chk(L.load_mhlik().mhlik_q8_quantize(x.data_ptr(), _TYPES[x.dtype], rows, cols, rs, cs, data.data_ptr(), scale.data_ptr(),
-                                          x.device.index, _stream(x.device)))
-    return Block8(data, scale, cols)
+    index = device.index
+    _chk(L.load_mhlik().mhlik_q8_quantize(x.data_ptr(), _TYPES[x.dtype], rows, cols, rs, cs, q.data.data_ptr(), q.scale.data_ptr(),
+                                          index, _stream(index)))
+    return q
+
+
+@functools.lru_cache(maxsize=256)
+def _product_space(rows, cols):
+    need = C.c_size_t()
+    _chk(L.load_mhlik().mhlik_q8_product_workspace(rows, cols, C.byref(need)))
+    return need.value
 
 
 def product(x, w, dtype=torch.float32):
@@ -100,42 +111,48 @@ def product(x, w, dtype=torch.float32):
     _need(isinstance(w, Block8), "w must be a Block8 (quantize it once)")
     _need(dtype in _OUT, "dtype is %s; wanted: %s", dtype, ", ".join(str(t) for t in _OUT))
     p = L.Q8Operands()
-    device = w.data.device
+    device = w.device
     if isinstance(x, Block8):
-        _same("x", x.data, device)
+        _same("x", x.device, device)
         rows, cols = x.rows, x.cols
         p.x, p.x_scale, p.x_type = x.data.data_ptr(), x.scale.data_ptr(), L.T_Q8
     else:
-        _given("x", x, 2, _TYPES)
-        _same("x", x, device)
+        _same("x", _given("x", x, 2, _TYPES), device)
         rows, cols = x.shape
         p.x, p.x_type = x.data_ptr(), _TYPES[x.dtype]
         p.x_row_stride, p.x_col_stride = x.stride()
-    _need(cols == w.cols, "x has %d columns, w has %d", cols, w.cols)
+    if cols != w.cols:
+        raise ValueError("x has %d columns, w has %d" % (cols, w.cols))
     if p.x_type != L.T_Q8:
-        p.workspace_bytes = rows * (w.data.shape[1] + w.scale.shape[1])
-        space = torch.empty(p.workspace_bytes, dtype=torch.uint8, device=device)
-        p.workspace = space.data_ptr()
-    out = torch.empty(rows, w.rows, dtype=dtype, device=device)
+        need = _product_space(rows, cols)
+        if need:
+            space = torch.empty(need, dtype=torch.uint8, device=device)
+            p.workspace, p.workspace_bytes = space.data_ptr(), need
+    draws = w.rows
+    out = torch.empty((rows, draws), dtype=dtype, device=device)
     p.w_data, p.w_scale, p.out = w.data.data_ptr(), w.scale.data_ptr(), out.data_ptr()
-    p.out_stride, p.out_type = w.rows, _OUT[dtype]
-    p.rows, p.draws, p.cols = rows, w.rows, cols
-    _chk(L.load_mhlik().mhlik_q8_product(C.byref(p), device.index, _stream(device)))
+    p.out_stride, p.out_type = draws, _OUT[dtype]
+    p.rows, p.draws, p.cols = rows, draws, cols
+    index = device.index
+    _chk(L.load_mhlik().mhlik_q8_product(C.byref(p), index, _stream(index)))
     return out
 
 
-def _choice(p, name, value, off, dtype, rows, device, held):
-    if value is None:
-        value = off
-    if isinstance(value, torch.Tensor):
-        _given(name, value, 1, (dtype,))
-        _same(name, value, device)
-        _need(value.shape[0] == rows, "%s has %d values for %d rows", name, value.shape[0], rows)
-        value = value.contiguous()
-        held.append(value)
-        setattr(p, name, value.data_ptr())
-    else:
-        setattr(p, name + "_all", value)
+def _each(name, value, kind, rows, device):
+    """A choice that every row has its own of."""
+    _same(name, _given(name, value, 1, kind), device)
+    _need(value.shape[0] == rows, "%s has %d values for %d rows", name, value.shape[0], rows)
+    return value.contiguous()
+
+
+_F32, _I32 = {torch.float32: None}, {torch.int32: None}
+
+
+@functools.lru_cache(maxsize=256)
+def _draw_space(rows, n):
+    need = C.c_size_t()
+    _chk(L.load_mhlik().mhlik_draw_workspace(rows, n, C.byref(need)))
+    return need.value
 
 
 def draw(z, u, temperature=1.0, top_k=None, top_p=None, min_p=None):
@@ -147,31 +164,47 @@ def draw(z, u, temperature=1.0, top_k=None, top_p=None, min_p=None):
     the first, in column order, at which the kept mass exceeds u of the whole.  temperature 0 takes the largest.  The
     four choices are numbers, or tensors of one value a row (float32; top_k int32); None is off, and so are top_k <= 0,
     top_p >= 1, min_p <= 0.  A row with nothing to draw (all -inf, or a NaN) gives column -1 and NaN."""
-    _given("z", z, 2, _OUT)
-    _given("u", u, 1, _U)
+    device = _given("z", z, 2, _OUT)
+    _same("u", _given("u", u, 1, _U), device)
     rows, n = z.shape
-    device = z.device
-    _same("u", u, device)
     _need(n >= 1, "z must have at least one column")
     _need(u.shape[0] == rows, "u has %d values for %d rows", u.shape[0], rows)
-    if z.stride(1) != 1 and n > 1:
+    stride, step = z.stride()
+    if step != 1 and n > 1:
         z = z.contiguous()
-    u = u.contiguous()
+        stride = n
+    if not u.is_contiguous():
+        u = u.contiguous()
     p = L.DrawRows()
-    held = []
-    _choice(p, "temperature", temperature, 1.0, torch.float32, rows, device, held)
-    _choice(p, "top_k", top_k, 0, torch.int32, rows, device, held)
-    _choice(p, "top_p", top_p, 1.0, torch.float32, rows, device, held)
-    _choice(p, "min_p", min_p, 0.0, torch.float32, rows, device, held)
+    if isinstance(temperature, torch.Tensor):
+        temperature = _each("temperature", temperature, _F32, rows, device)
+        p.temperature = temperature.data_ptr()
+    else:
+        p.temperature_all = 1.0 if temperature is None else temperature
+    if isinstance(top_k, torch.Tensor):
+        top_k = _each("top_k", top_k, _I32, rows, device)
+        p.top_k = top_k.data_ptr()
+    elif top_k is not None:
+        p.top_k_all = max(0, min(top_k, n))
+    if isinstance(top_p, torch.Tensor):
+        top_p = _each("top_p", top_p, _F32, rows, device)
+        p.top_p = top_p.data_ptr()
+    else:
+        p.top_p_all = 1.0 if top_p is None else top_p
+    if isinstance(min_p, torch.Tensor):
+        min_p = _each("min_p", min_p, _F32, rows, device)
+        p.min_p = min_p.data_ptr()
+    elif min_p is not None:
+        p.min_p_all = min_p
     index = torch.empty(rows, dtype=torch.int64, device=device)
     logp = torch.empty(rows, dtype=torch.float32, device=device)
-    p.z, p.rows, p.n, p.stride, p.z_type = z.data_ptr(), rows, n, z.stride(0), _OUT[z.dtype]
+    p.z, p.rows, p.n, p.stride, p.z_type = z.data_ptr(), rows, n, stride, _OUT[z.dtype]
     p.u, p.u_type = u.data_ptr(), _U[u.dtype]
     p.index, p.logp = index.data_ptr(), logp.data_ptr()
-    need = C.c_size_t()
-    _chk(L.load_mhlik().mhlik_draw_workspace(rows, n, C.byref(need)))
-    if need.value:
-        space = torch.empty(need.value, dtype=torch.uint8, device=device)
-        p.workspace, p.workspace_bytes = space.data_ptr(), need.value
-    _chk(L.load_mhlik().mhlik_draw(C.byref(p), device.index, _stream(device)))
+    need = _draw_space(rows, n)
+    if need:
+        space = torch.empty(need, dtype=torch.uint8, device=device)
+        p.workspace, p.workspace_bytes = space.data_ptr(), need
+    gpu = device.index
+    _chk(L.load_mhlik().mhlik_draw(C.byref(p), gpu, _stream(gpu)))
     return index, logp
