@@ -112,13 +112,6 @@ template <int BINS> struct DrawBin {
 
 __device__ __forceinline__ unsigned long long draw_fixed(double w, int shift) { return (unsigned long long)rint(ldexp(w, shift)); }
 
-__device__ __forceinline__ double draw_wave_sum(double v)
-{
-#pragma unroll
-  for (int d = 1; d < kWave; d <<= 1) v += __shfl_xor(v, d);
-  return v;
-}
-
 // Position in the order: smaller is earlier (larger value, lower column).
 __device__ __forceinline__ unsigned long long draw_place(float z, int j)
 {
@@ -142,7 +135,7 @@ __device__ int draw_pick(const double (&w)[VPT], double aim, double *total, doub
   double m = 0.0;
 #pragma unroll
   for (int i = 0; i < VPT; i++) m += w[i];
-  m = draw_wave_sum(m);
+  m = wave_sum(m);
   __syncthreads();
   if (lane == 0) lds[wave] = m;
   __syncthreads();
@@ -173,7 +166,7 @@ __device__ int draw_pick(const double (&w)[VPT], double aim, double *total, doub
     bool done = false;
 #pragma unroll
     for (int i = 0; i < VPT; i++) { // the same for the runs of 64
-      const double v = draw_wave_sum(w[i]);
+      const double v = wave_sum(w[i]);
       if (!done && v > 0.0) {
         at = i;
         before = sum;
@@ -183,12 +176,7 @@ __device__ int draw_pick(const double (&w)[VPT], double aim, double *total, doub
       sum += v;
     }
     aim -= before;
-    double run = mine;
-#pragma unroll
-    for (int d = 1; d < kWave; d <<= 1) {
-      const double b = __shfl_up(run, d);
-      if (lane >= d) run += b;
-    }
+    const double run = wave_running(mine);
     const unsigned long long over = __ballot(mine > 0.0 && run > aim), some = __ballot(mine > 0.0);
     const int who = over ? __ffsll(over) - 1 : 63 - __clzll((long long)some);
     if (lane == who) {
@@ -270,18 +258,9 @@ __device__ void draw_narrow(DrawRow<T> &r, DrawShared &s, int shift, uint32_t k,
       cn += s.count[top - i];
       if (BY_MASS) cm += s.mass[top - i];
     }
-    uint32_t in = cn;
-    unsigned long long im = cm;
+    const uint32_t in = wave_running(cn);
+    const unsigned long long im = wave_running(cm);
     const int lane = tid % kWave;
-#pragma unroll
-    for (int d = 1; d < kWave; d <<= 1) {
-      const uint32_t a = __shfl_up(in, d);
-      const unsigned long long b = __shfl_up(im, d);
-      if (lane >= d) {
-        in += a;
-        im += b;
-      }
-    }
     if (lane == kWave - 1) {
       s.i[tid / kWave] = in;
       s.q[tid / kWave] = im;
@@ -408,11 +387,11 @@ template <int THREADS> struct ShortShared {
   uint32_t i[32];
 };
 
-// Narrows the kept prefix.  z: -inf where there is nothing; column j of z[i] from at(i).  Returns false if a border's
+// Narrows the kept prefix.  z: -inf where there is nothing; column j of z[i] from at(i); weight: of z[i].  Returns false if a border's
 // bin holds more values than there is room for.
 template <int THREADS, int VPT, typename AT>
-__device__ bool draw_short_narrow(const float (&z)[VPT], AT at, float max, float min, const DrawChoice &c, int shift,
-                                  ShortShared<THREADS> &s, DrawEnd *end)
+__device__ bool draw_short_narrow(const float (&z)[VPT], const double (&weight)[VPT], AT at, float max, float min, const DrawChoice &c,
+                                  int shift, ShortShared<THREADS> &s, DrawEnd *end)
 {
   constexpr int kWaves = THREADS / kWave, kRun = kShortBins / THREADS;
   const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
@@ -430,7 +409,7 @@ __device__ bool draw_short_narrow(const float (&z)[VPT], AT at, float max, float
       const int b = bin.of(z[i]);
       atomicAdd(&s.count[b], 1u);
       if (by_mass) {
-        const unsigned long long m = draw_fixed(draw_weight(z[i], max, c.inv_t), shift);
+        const unsigned long long m = draw_fixed(weight[i], shift);
         if (m) atomicAdd(&s.mass[b], m);
       }
     }
@@ -443,17 +422,8 @@ __device__ bool draw_short_narrow(const float (&z)[VPT], AT at, float max, float
     cn += s.count[tid * kRun + i];
     cm += s.mass[tid * kRun + i];
   }
-  uint32_t in = cn;
-  unsigned long long im = cm;
-#pragma unroll
-  for (int d = 1; d < kWave; d <<= 1) {
-    const uint32_t a = __shfl_up(in, d);
-    const unsigned long long b = __shfl_up(im, d);
-    if (lane >= d) {
-      in += a;
-      im += b;
-    }
-  }
+  uint32_t in = wave_running(cn);
+  unsigned long long im = wave_running(cm);
   if (lane == kWave - 1) {
     s.i[wave] = in;
     s.q[wave] = im;
@@ -501,7 +471,7 @@ __device__ bool draw_short_narrow(const float (&z)[VPT], AT at, float max, float
         const uint32_t q = atomicAdd(&s.i[30], 1u);
         if (q < ShortShared<THREADS>::kCap) {
           s.place[q] = draw_place(z[i], at(i));
-          s.cmass[q] = by_mass ? draw_fixed(draw_weight(z[i], max, c.inv_t), shift) : 0;
+          s.cmass[q] = by_mass ? draw_fixed(weight[i], shift) : 0;
         }
       }
     __syncthreads();
@@ -627,11 +597,8 @@ template <typename T, int THREADS, int VPT> __global__ __launch_bounds__(THREADS
     if (z[i] > -HUGE_VALF) min = fminf(min, z[i]);
   }
   const DrawChoice c = draw_choice(a, row);
-#pragma unroll
-  for (int d = 1; d < kWave; d <<= 1) {
-    max = fmaxf(max, __shfl_xor(max, d));
-    min = fminf(min, __shfl_xor(min, d));
-  }
+  max = wave_max(max);
+  min = wave_min(min);
   const bool any = __any(nan);
   if (lane == 0) {
     s.quick.f[wave] = max;
@@ -663,15 +630,15 @@ template <typename T, int THREADS, int VPT> __global__ __launch_bounds__(THREADS
     if (tid == 0) draw_answer(a, row, s.quick.i[0], 0.0);
     return;
   }
-  DrawEnd end{~0ull};
-  if (c.k || c.share < 1.0)
-    if (!draw_short_narrow<THREADS, VPT>(z, at, max, min, c, shift, s.quick, &end)) end = draw_whole<T, THREADS>(a, row, c, max, shift, s.whole);
   double w[VPT];
 #pragma unroll
-  for (int i = 0; i < VPT; i++) {
-    w[i] = z[i] > -HUGE_VALF && end.kept(z[i], at(i)) ? draw_weight(z[i], max, c.inv_t) : 0.0;
-    if (w[i] < c.least) w[i] = 0.0;
-  }
+  for (int i = 0; i < VPT; i++) w[i] = draw_weight(z[i], max, c.inv_t);
+  DrawEnd end{~0ull};
+  if (c.k || c.share < 1.0)
+    if (!draw_short_narrow<THREADS, VPT>(z, w, at, max, min, c, shift, s.quick, &end)) end = draw_whole<T, THREADS>(a, row, c, max, shift, s.whole);
+#pragma unroll
+  for (int i = 0; i < VPT; i++)
+    if (!end.kept(z[i], at(i)) || w[i] < c.least) w[i] = 0.0;
   double total, weight, rest;
   __syncthreads();
   const int place = draw_pick<THREADS, VPT, true>(w, c.u, &total, &weight, &rest, s.quick.d);
@@ -745,13 +712,8 @@ __device__ inline void draw_row_range(const LongPart *part, int units, float *ma
     b = fminf(b, part[q].min);
     bad |= part[q].nan;
   }
-#pragma unroll
-  for (int d = 1; d < kWave; d <<= 1) {
-    a = fmaxf(a, __shfl_xor(a, d));
-    b = fminf(b, __shfl_xor(b, d));
-  }
-  *max = a;
-  *min = b;
+  *max = wave_max(a);
+  *min = wave_min(b);
   *nan = __any(bad) != 0;
 }
 
@@ -803,11 +765,8 @@ __global__ __launch_bounds__(kBlock) void draw_top_kernel(DrawArgs a, LongSpace 
     max = fmaxf(max, z[i]);
     if (z[i] > -HUGE_VALF) min = fminf(min, z[i]);
   }
-#pragma unroll
-  for (int d = 1; d < kWave; d <<= 1) {
-    max = fmaxf(max, __shfl_xor(max, d));
-    min = fminf(min, __shfl_xor(min, d));
-  }
+  max = wave_max(max);
+  min = wave_min(min);
   const DrawChoice c = draw_choice(a, row);
   int first = INT32_MAX;
   double mass = 0.0;
@@ -815,15 +774,11 @@ __global__ __launch_bounds__(kBlock) void draw_top_kernel(DrawArgs a, LongSpace 
 #pragma unroll
     for (int i = VPT - 1; i >= 0; i--)
       if (z[i] == max) first = draw_column<VEC>(base, i);
-#pragma unroll
-    for (int d = 1; d < kWave; d <<= 1) {
-      const int o = __shfl_xor(first, d);
-      first = o < first ? o : first;
-    }
+    first = (int)wave_min((uint32_t)first);
   } else if (draw_kind(c, false, max) == kRowPlain) {
 #pragma unroll
     for (int i = 0; i < VPT; i++) mass += draw_weight(z[i], max, c.inv_t);
-    mass = draw_wave_sum(mass);
+    mass = wave_sum(mass);
   }
   const bool any = __any(nan);
   if (lane == 0) g.part[row * g.units + unit] = LongPart{max, min, first, any, mass};
@@ -883,12 +838,7 @@ __global__ __launch_bounds__(kBlock) void draw_collect_kernel(DrawArgs a, LongSp
       h[i] = g.histo[row * kLongBins + tid * kRun + i];
       mine += h[i];
     }
-    unsigned long long in = mine;
-#pragma unroll
-    for (int d = 1; d < kWave; d <<= 1) {
-      const unsigned long long b = __shfl_up(in, d);
-      if (lane >= d) in += b;
-    }
+    unsigned long long in = wave_running(mine);
     if (lane == kWave - 1) sums[wave] = in;
     if (tid == 0) cell = LongCell{kLongBins - 1, 0, 0, 0.0};
     __syncthreads();
@@ -954,7 +904,7 @@ __global__ __launch_bounds__(kBlock) void draw_collect_kernel(DrawArgs a, LongSp
       }
     n += total;
   }
-  kept = draw_wave_sum(kept);
+  kept = wave_sum(kept);
   if (lane == 0) {
     g.kept[row * g.units + u] = kept;
     g.listed[row * g.units + u] = n;
@@ -987,11 +937,7 @@ template <typename T, int VPT> __global__ __launch_bounds__(1024) void draw_fini
       int first = INT32_MAX;
       for (int q = lane; q < g.units; q += kWave)
         if (part[q].max == max && part[q].first < first) first = part[q].first;
-#pragma unroll
-      for (int d = 1; d < kWave; d <<= 1) {
-        const int o = __shfl_xor(first, d);
-        first = o < first ? o : first;
-      }
+      first = (int)wave_min((uint32_t)first);
       if (lane == 0) draw_answer(a, row, first, 0.0);
     }
     return;
@@ -1007,12 +953,7 @@ template <typename T, int VPT> __global__ __launch_bounds__(1024) void draw_fini
     if (!whole) {
       mine = tid < g.units ? g.listed[row * g.units + tid] : 0;
       if (mine > kUnit / 2) mine = kLongList + 1; // the unit's list is too short
-      in = mine;
-#pragma unroll
-      for (int d = 1; d < kWave; d <<= 1) {
-        const int b = __shfl_up(in, d);
-        if (lane >= d) in += b;
-      }
+      in = (int)wave_running((uint32_t)mine);
       if (lane == kWave - 1) s.quick.i[wave] = (uint32_t)in;
       __syncthreads();
       for (int w = 0; w < kThreads / kWave; w++) {
@@ -1039,13 +980,13 @@ template <typename T, int VPT> __global__ __launch_bounds__(1024) void draw_fini
     auto at = [&](int i) { return list[place_of(i)].j; };
 #pragma unroll
     for (int i = 0; i < kList; i++) z[i] = place_of(i) < listed ? list[place_of(i)].z : -HUGE_VALF;
-    if (draw_short_narrow<kThreads, kList>(z, at, max, min, c, shift, s.quick, &end)) {
-      double w[kList];
+    double w[kList];
 #pragma unroll
-      for (int i = 0; i < kList; i++) {
-        w[i] = z[i] > -HUGE_VALF && end.kept(z[i], at(i)) ? draw_weight(z[i], max, c.inv_t) : 0.0;
-        if (w[i] < c.least) w[i] = 0.0;
-      }
+    for (int i = 0; i < kList; i++) w[i] = draw_weight(z[i], max, c.inv_t);
+    if (draw_short_narrow<kThreads, kList>(z, w, at, max, min, c, shift, s.quick, &end)) {
+#pragma unroll
+      for (int i = 0; i < kList; i++)
+        if (!end.kept(z[i], at(i)) || w[i] < c.least) w[i] = 0.0;
       double total, weight, rest;
       __syncthreads();
       const int place = draw_pick<kThreads, kList, true>(w, c.u, &total, &weight, &rest, s.quick.d);
@@ -1093,7 +1034,7 @@ template <typename T, int VPT> __global__ __launch_bounds__(1024) void draw_fini
         const int j = q * kUnit + i * kWave + lane;
         if (j < n) v += weight_of((float)zp[j], j);
       }
-      v = draw_wave_sum(v);
+      v = wave_sum(v);
       if (lane == 0) g.kept[row * g.units + q] = v;
     }
     __threadfence_block();
@@ -1147,8 +1088,7 @@ template <typename T> __global__ __launch_bounds__(1024) void draw_huge_kernel(D
     nan |= z != z;
     max = fmaxf(max, z);
   }
-#pragma unroll
-  for (int d = 1; d < kWave; d <<= 1) max = fmaxf(max, __shfl_xor(max, d));
+  max = wave_max(max);
   const bool any = __any(nan);
   if (lane == 0) {
     s.f[wave] = max;
@@ -1190,7 +1130,7 @@ template <typename T> __global__ __launch_bounds__(1024) void draw_huge_kernel(D
     const int64_t lo = from + wave * run < to ? from + wave * run : to, hi = lo + run < to ? lo + run : to;
     double m = 0.0;
     for (int64_t j = lo + lane; j < hi; j += kWave) m += weight_of((int)j);
-    m = draw_wave_sum(m);
+    m = wave_sum(m);
     __syncthreads();
     if (lane == 0) s.d[wave] = m;
     __syncthreads();
@@ -1215,12 +1155,7 @@ template <typename T> __global__ __launch_bounds__(1024) void draw_huge_kernel(D
   }
   if (wave == 0) {
     const double w = lane < to - from ? weight_of((int)from + lane) : 0.0;
-    double m = w;
-#pragma unroll
-    for (int d = 1; d < kWave; d <<= 1) {
-      const double b = __shfl_up(m, d);
-      if (lane >= d) m += b;
-    }
+    const double m = wave_running(w);
     const unsigned long long over = __ballot(w > 0.0 && m > aim), some = __ballot(w > 0.0);
     const int pick = over ? __ffsll(over) - 1 : 63 - __clzll((long long)some);
     if (lane == pick) draw_answer(a, row, from + lane, log(w / total));

@@ -2,11 +2,74 @@
 #pragma once
 
 #include <hip/hip_runtime.h>
+#include <math.h>
 #include <stdint.h>
 
 namespace mhlik {
 
 constexpr int kBlock = 256; // threads per workgroup (4 waves) unless a kernel says otherwise
 constexpr int kWave = 64;
+
+// ---- sums and maxima over a wave with DPP moves (no LDS, a tenth of a shuffle's latency): row_shr 1, 2, 4, 8 scan each 16
+// lanes, row_bcast 15 and 31 carry the totals on.  A lane without a source reads the identity.
+
+template <int CTRL, int ROWS> __device__ __forceinline__ uint32_t dpp_move(uint32_t v, uint32_t identity)
+{
+  return (uint32_t)__builtin_amdgcn_update_dpp((int)identity, (int)v, CTRL, ROWS, 0xf, false);
+}
+template <int CTRL, int ROWS> __device__ __forceinline__ float dpp_move(float v, float identity)
+{
+  return __uint_as_float(dpp_move<CTRL, ROWS>(__float_as_uint(v), __float_as_uint(identity)));
+}
+template <int CTRL, int ROWS> __device__ __forceinline__ unsigned long long dpp_move(unsigned long long v, unsigned long long identity)
+{
+  const uint32_t lo = dpp_move<CTRL, ROWS>((uint32_t)v, (uint32_t)identity), hi = dpp_move<CTRL, ROWS>((uint32_t)(v >> 32), (uint32_t)(identity >> 32));
+  return (unsigned long long)hi << 32 | lo;
+}
+template <int CTRL, int ROWS> __device__ __forceinline__ double dpp_move(double v, double identity)
+{
+  return __longlong_as_double((long long)dpp_move<CTRL, ROWS>((unsigned long long)__double_as_longlong(v), (unsigned long long)__double_as_longlong(identity)));
+}
+
+template <typename V, typename OP> __device__ __forceinline__ V wave_scan(V v, V identity, OP op)
+{
+  v = op(v, dpp_move<0x111, 0xf>(v, identity));
+  v = op(v, dpp_move<0x112, 0xf>(v, identity));
+  v = op(v, dpp_move<0x114, 0xf>(v, identity));
+  v = op(v, dpp_move<0x118, 0xf>(v, identity));
+  v = op(v, dpp_move<0x142, 0xa>(v, identity));
+  v = op(v, dpp_move<0x143, 0xc>(v, identity));
+  return v;
+}
+
+__device__ __forceinline__ uint32_t wave_last(uint32_t v) { return (uint32_t)__builtin_amdgcn_readlane((int)v, kWave - 1); }
+__device__ __forceinline__ float wave_last(float v) { return __uint_as_float(wave_last(__float_as_uint(v))); }
+__device__ __forceinline__ unsigned long long wave_last(unsigned long long v)
+{
+  return (unsigned long long)wave_last((uint32_t)(v >> 32)) << 32 | wave_last((uint32_t)v);
+}
+__device__ __forceinline__ double wave_last(double v)
+{
+  return __longlong_as_double((long long)wave_last((unsigned long long)__double_as_longlong(v)));
+}
+
+// Running sum over the lanes up to and with this one.
+template <typename V> __device__ __forceinline__ V wave_running(V v)
+{
+  return wave_scan(v, (V)0, [](V a, V b) { return a + b; });
+}
+template <typename V> __device__ __forceinline__ V wave_sum(V v) { return wave_last(wave_running(v)); }
+__device__ __forceinline__ float wave_max(float v)
+{
+  return wave_last(wave_scan(v, -HUGE_VALF, [](float a, float b) { return fmaxf(a, b); }));
+}
+__device__ __forceinline__ float wave_min(float v)
+{
+  return wave_last(wave_scan(v, HUGE_VALF, [](float a, float b) { return fminf(a, b); }));
+}
+__device__ __forceinline__ uint32_t wave_min(uint32_t v)
+{
+  return wave_last(wave_scan(v, 0xffffffffu, [](uint32_t a, uint32_t b) { return a < b ? a : b; }));
+}
 
 } // namespace mhlik
