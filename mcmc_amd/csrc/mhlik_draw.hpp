@@ -49,17 +49,44 @@ __device__ __forceinline__ float draw_value(uint32_t key)
   return __uint_as_float(key ^ (key >> 31 ? 0x80000000u : 0xffffffffu));
 }
 
-// exp((z - max) / T); z = max: 1, also for infinite max; -800 underflows to 0, and fmax takes NaN (-inf * 0) there too
-__device__ __forceinline__ double draw_weight(float z, float max, double inv_t)
-{
-  const double d = z == max ? 0.0 : (double)z - (double)max;
-  return z == -HUGE_VALF ? 0.0 : mhlik_exp_fast(fmax(d * inv_t, -800.0));
-}
+// A log weight as the kernels see it: +inf counts as the largest float, so that differences exist.
+__device__ __forceinline__ float draw_finite(float z) { return fminf(z, 0x1.fffffep127f); }
 
+// 2^((z - max) s), s = log2(e) / T: 1 at z = max, within 5e-16 relative where it matters ((z - max) s is rounded: another
+// 1e-16 times itself), 0 below 2^-1020 and for z = -inf.  Whole part by adding 1.5 * 2^52, whose low bits then hold it;
+// the rest goes through the degree-10 polynomial of mhlik_exp_fast with the powers of ln 2 multiplied in: 17 double
+// instructions, of which none is slower than an addition.
+__device__ __forceinline__ double draw_weight(float z, float max, double s)
+{
+  MHLIK_SP_COEF(c10, 0x1.e364ae3ebe671p-28);
+  MHLIK_SP_COEF(c9, 0x1.b660a93518429p-24);
+  MHLIK_SP_COEF(c8, 0x1.62c1651329726p-20);
+  MHLIK_SP_COEF(c7, 0x1.ffcb6d52a8ae3p-17);
+  MHLIK_SP_COEF(c6, 0x1.4309126702394p-13);
+  MHLIK_SP_COEF(c5, 0x1.5d87fe93109eep-10);
+  MHLIK_SP_COEF(c4, 0x1.3b2ab6fbd4a75p-7);
+  MHLIK_SP_COEF(c3, 0x1.c6b08d704396dp-5);
+  MHLIK_SP_COEF(c2, 0x1.ebfbdff82c46cp-3);
+  MHLIK_SP_COEF(c1, 0x1.62e42fefa39efp-1);
+  const double y = fmax(((double)z - (double)max) * s, -1100.0); // NaN (-inf * 0) too
+  const double m = y + 0x1.8p52, f = y - (m - 0x1.8p52);
+  double p = fma(c10, f, c9);
+  p = fma(p, f, c8);
+  p = fma(p, f, c7);
+  p = fma(p, f, c6);
+  p = fma(p, f, c5);
+  p = fma(p, f, c4);
+  p = fma(p, f, c3);
+  p = fma(p, f, c2);
+  p = fma(p, f, c1);
+  p = fma(p, f, 1.0);
+  const double w = __hiloint2double(__double2hiint(p) + (int)((uint32_t)__double2loint(m) << 20), __double2loint(p));
+  return y < -1020.0 ? 0.0 : w;
+}
 
 // The choices of one row.
 struct DrawChoice {
-  double temp, inv_t, share, least, u; // least: at most 1
+  double temp, rate, share, least, u; // rate: log2(e) / temp; least: at most 1
   int k;                               // 0: no top-k
   bool bad, greedy;                    // a choice that is not a number; temperature 0
 };
@@ -75,7 +102,7 @@ __device__ inline DrawChoice draw_choice(const DrawArgs &a, int64_t row)
   if (c.k <= 0 || c.k >= a.n) c.k = 0;
   c.bad = !(c.temp >= 0.0) || c.share != c.share || c.least != c.least || c.u != c.u;
   c.greedy = c.temp == 0.0;
-  c.inv_t = c.greedy ? 1.0 : 1.0 / c.temp;
+  c.rate = c.greedy ? 1.0 : 1.4426950408889634074 / c.temp;
   c.share = c.share > 0.0 ? c.share : 0.0;
   if (c.least > 1.0) c.least = 1.0;
   return c;
@@ -106,7 +133,7 @@ template <int BINS> struct DrawBin {
   }
   __device__ __forceinline__ int of(float z) const
   {
-    return z == max ? 0 : (int)fminf((max - z) * scale, (float)(BINS - 1));
+    return (int)fminf((max - z) * scale, (float)(BINS - 1));
   }
 };
 
@@ -210,10 +237,10 @@ template <typename T> struct DrawRow {
   const T *z;
   int n;
   float max;
-  double inv_t;
+  double rate;
   uint32_t key; // kept: larger keys, and equal ones up to column `last`
   int last;
-  __device__ __forceinline__ float at(int j) const { return (float)z[j]; }
+  __device__ __forceinline__ float at(int j) const { return draw_finite((float)z[j]); }
   __device__ __forceinline__ bool kept(uint32_t k, int j) const { return k > key || (k == key && j <= last); }
 };
 
@@ -244,7 +271,7 @@ __device__ void draw_narrow(DrawRow<T> &r, DrawShared &s, int shift, uint32_t k,
       const uint32_t bin = (key >> low) & ((1u << bits) - 1);
       atomicAdd(&s.count[bin], 1u);
       if (BY_MASS) {
-        const unsigned long long m = (unsigned long long)rint(ldexp(draw_weight(z, r.max, r.inv_t), shift));
+        const unsigned long long m = (unsigned long long)rint(ldexp(draw_weight(z, r.max, r.rate), shift));
         if (m) atomicAdd(&s.mass[bin], m);
       }
     }
@@ -322,7 +349,7 @@ __device__ void draw_narrow(DrawRow<T> &r, DrawShared &s, int shift, uint32_t k,
   // `prefix` is the key now; of its `equal` columns the first `take` are needed
   uint32_t take;
   if (BY_MASS) {
-    const double w = draw_weight(draw_value(prefix), r.max, r.inv_t), a = (double)above_m * unit;
+    const double w = draw_weight(draw_value(prefix), r.max, r.rate), a = (double)above_m * unit;
     const double c = w > 0.0 ? ceil((target - a) / w) : 1.0;
     take = c < 1.0 ? 1u : c > (double)equal ? equal : (uint32_t)c;
     if (take > 1 && a + (take - 1) * w >= target) take--;
@@ -374,11 +401,11 @@ __device__ void draw_narrow(DrawRow<T> &r, DrawShared &s, int shift, uint32_t k,
 // (counts and masses) gives the bin in which a border falls; the few values of that bin go to LDS and each finds its
 // rank, and the mass before it, by comparing with all others.
 
-constexpr int kShortBins = 1024;
 template <int THREADS> struct ShortShared {
   static constexpr int kCap = THREADS; // values of a border's bin
-  unsigned long long mass[kShortBins];
-  uint32_t count[kShortBins];
+  static constexpr int kBins = THREADS == 1024 ? 1024 : 512;
+  unsigned long long mass[kBins];
+  uint32_t count[kBins];
   unsigned long long place[kCap];
   unsigned long long cmass[kCap];
   double d[32];
@@ -393,7 +420,7 @@ template <int THREADS, int VPT, typename AT>
 __device__ bool draw_short_narrow(const float (&z)[VPT], const double (&weight)[VPT], AT at, float max, float min, const DrawChoice &c,
                                   int shift, ShortShared<THREADS> &s, DrawEnd *end)
 {
-  constexpr int kWaves = THREADS / kWave, kRun = kShortBins / THREADS;
+  constexpr int kWaves = THREADS / kWave, kShortBins = ShortShared<THREADS>::kBins, kRun = kShortBins / THREADS;
   const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
   const DrawBin<kShortBins> bin(max, min, c.temp);
   const bool by_mass = c.share < 1.0;
@@ -567,7 +594,7 @@ __device__ DrawEnd draw_whole(const DrawArgs &a, int64_t row, const DrawChoice &
   r.z = (const T *)a.z + row * a.stride;
   r.n = (int)a.n;
   r.max = max;
-  r.inv_t = c.inv_t;
+  r.rate = c.rate;
   r.key = 0;
   r.last = r.n;
   __syncthreads();
@@ -591,8 +618,9 @@ template <typename T, int THREADS, int VPT> __global__ __launch_bounds__(THREADS
   bool nan = false;
 #pragma unroll
   for (int i = 0; i < VPT; i++) {
-    z[i] = at(i) < n ? (float)zp[at(i)] : -HUGE_VALF;
-    nan |= z[i] != z[i];
+    const float v = at(i) < n ? (float)zp[at(i)] : -HUGE_VALF;
+    nan |= v != v;
+    z[i] = draw_finite(v);
     max = fmaxf(max, z[i]);
     if (z[i] > -HUGE_VALF) min = fminf(min, z[i]);
   }
@@ -632,7 +660,7 @@ template <typename T, int THREADS, int VPT> __global__ __launch_bounds__(THREADS
   }
   double w[VPT];
 #pragma unroll
-  for (int i = 0; i < VPT; i++) w[i] = draw_weight(z[i], max, c.inv_t);
+  for (int i = 0; i < VPT; i++) w[i] = draw_weight(z[i], max, c.rate);
   DrawEnd end{~0ull};
   if (c.k || c.share < 1.0)
     if (!draw_short_narrow<THREADS, VPT>(z, w, at, max, min, c, shift, s.quick, &end)) end = draw_whole<T, THREADS>(a, row, c, max, shift, s.whole);
@@ -657,7 +685,7 @@ template <typename T, int THREADS, int VPT> __global__ __launch_bounds__(THREADS
 //   finish   one workgroup a row: the border among the listed values, the unit in which the kept mass exceeds u of the
 //            whole, the column in it.  A row whose lists are too long goes the whole-row way.
 
-constexpr int kLongBins = 2048;
+constexpr int kLongBins = 512;
 constexpr int kLongList = 2048;  // listed values of a row
 constexpr int kLongUnits = 1024; // units of a row: one a thread of the finishing workgroup
 
@@ -717,10 +745,12 @@ __device__ inline void draw_row_range(const LongPart *part, int units, float *ma
   *nan = __any(bad) != 0;
 }
 
-// A unit's values: register v * VEC + e of lane l holds column base + (v * 64 + l) * VEC + e; -inf past the end.
-template <typename T, int VEC, int VPT> __device__ __forceinline__ void draw_load(const T *row, int n, int base, float (&z)[VPT])
+// A unit's values: register v * VEC + e of lane l holds column base + (v * 64 + l) * VEC + e; -inf past the end.  True if
+// one of them is NaN.
+template <typename T, int VEC, int VPT> __device__ __forceinline__ bool draw_load(const T *row, int n, int base, float (&z)[VPT])
 {
-  struct alignas(sizeof(T) * VEC) Pack { T e[VEC]; };
+  bool nan = false;
+  struct __attribute__((packed, aligned(sizeof(T)))) Pack { T e[VEC]; }; // gfx950 takes unaligned accesses
   const int lane = threadIdx.x % kWave;
   if (base + VPT * kWave <= n) {
     Pack p[VPT / VEC];
@@ -739,6 +769,12 @@ template <typename T, int VEC, int VPT> __device__ __forceinline__ void draw_loa
         z[v * VEC + e] = j < n ? (float)row[j] : -HUGE_VALF;
       }
   }
+#pragma unroll
+  for (int i = 0; i < VPT; i++) {
+    nan |= z[i] != z[i];
+    z[i] = draw_finite(z[i]);
+  }
+  return nan;
 }
 template <int VEC> __device__ __forceinline__ int draw_column(int base, int i)
 {
@@ -756,12 +792,10 @@ __global__ __launch_bounds__(kBlock) void draw_top_kernel(DrawArgs a, LongSpace 
   if (unit >= g.units) return;
   const int base = unit * VPT * kWave;
   float z[VPT];
-  draw_load<T, VEC, VPT>((const T *)a.z + row * a.stride, (int)a.n, base, z);
+  const bool nan = draw_load<T, VEC, VPT>((const T *)a.z + row * a.stride, (int)a.n, base, z);
   float max = -HUGE_VALF, min = HUGE_VALF;
-  bool nan = false;
 #pragma unroll
   for (int i = 0; i < VPT; i++) {
-    nan |= z[i] != z[i];
     max = fmaxf(max, z[i]);
     if (z[i] > -HUGE_VALF) min = fminf(min, z[i]);
   }
@@ -777,7 +811,7 @@ __global__ __launch_bounds__(kBlock) void draw_top_kernel(DrawArgs a, LongSpace 
     first = (int)wave_min((uint32_t)first);
   } else if (draw_kind(c, false, max) == kRowPlain) {
 #pragma unroll
-    for (int i = 0; i < VPT; i++) mass += draw_weight(z[i], max, c.inv_t);
+    for (int i = 0; i < VPT; i++) mass += draw_weight(z[i], max, c.rate);
     mass = wave_sum(mass);
   }
   const bool any = __any(nan);
@@ -785,11 +819,11 @@ __global__ __launch_bounds__(kBlock) void draw_top_kernel(DrawArgs a, LongSpace 
 }
 
 template <typename T, int VEC, int VPT>
-__global__ __launch_bounds__(kBlock) void draw_histo_kernel(DrawArgs a, LongSpace g, int shift)
+__global__ __launch_bounds__(kBlock) void draw_histo_kernel(DrawArgs a, LongSpace g, int groups, int shift)
 {
   __shared__ unsigned long long bins[kLongBins];
-  const int64_t row = blockIdx.x / g.groups;
-  const int group = blockIdx.x % g.groups, wave = threadIdx.x / kWave;
+  const int64_t row = blockIdx.x / groups;
+  const int group = blockIdx.x % groups, wave = threadIdx.x / kWave;
   float max, min;
   bool nan;
   draw_row_range(g.part + row * g.units, g.units, &max, &min, &nan);
@@ -799,14 +833,13 @@ __global__ __launch_bounds__(kBlock) void draw_histo_kernel(DrawArgs a, LongSpac
   for (int b = threadIdx.x; b < kLongBins; b += kBlock) bins[b] = 0;
   __syncthreads();
   const DrawBin<kLongBins> bin(max, min, c.temp);
-  const int unit = group * 4 + wave;
-  if (unit < g.units) {
+  for (int unit = group * 4 + wave; unit < g.units; unit += groups * 4) {
     float z[VPT];
     draw_load<T, VEC, VPT>((const T *)a.z + row * a.stride, (int)a.n, unit * VPT * kWave, z);
 #pragma unroll
     for (int i = 0; i < VPT; i++)
       if (z[i] > -HUGE_VALF) {
-        const unsigned long long m = kind == kRowList ? 1 : draw_fixed(draw_weight(z[i], max, c.inv_t), shift);
+        const unsigned long long m = kind == kRowList ? 1 : draw_fixed(draw_weight(z[i], max, c.rate), shift);
         if (m) atomicAdd(&bins[bin.of(z[i])], m);
       }
   }
@@ -882,13 +915,13 @@ __global__ __launch_bounds__(kBlock) void draw_collect_kernel(DrawArgs a, LongSp
       const float x = z[v * VEC + e];
       take[e] = false;
       if (kind == kRowSums) {
-        const double w = draw_weight(x, max, c.inv_t);
+        const double w = draw_weight(x, max, c.rate);
         if (w >= c.least) kept += w;
       } else if (x > -HUGE_VALF) {
         const int b = bin.of(x);
         take[e] = kind == kRowList ? b <= border : b == border;
         if (kind == kRowNucleus && b < border) {
-          const double w = draw_weight(x, max, c.inv_t);
+          const double w = draw_weight(x, max, c.rate);
           if (w >= c.least) kept += w;
         }
       }
@@ -964,11 +997,14 @@ template <typename T, int VPT> __global__ __launch_bounds__(1024) void draw_fini
       __syncthreads();
       whole = listed > (kind == kRowList ? kLongList : kThreads);
     }
-    if (!whole) { // a wave brings a unit's list
-      for (int q = wave; q < g.units; q += kThreads / kWave) {
-        const int n = g.listed[row * g.units + q];
-        const LongCand *l = g.list + (row * g.units + q) * (kUnit / 2);
-        for (int i = lane; i < n; i += kWave) list[from[q] + i] = l[i];
+    if (!whole) { // each thread finds the unit of its entry: the last one that begins at or before it
+      for (int i = tid; i < listed; i += kThreads) {
+        int lo = 0, hi = g.units - 1;
+        while (lo < hi) {
+          const int mid = (lo + hi + 1) / 2;
+          if (from[mid] <= i) lo = mid; else hi = mid - 1;
+        }
+        list[i] = g.list[(row * g.units + lo) * (kUnit / 2) + i - from[lo]];
       }
       __syncthreads();
     }
@@ -982,7 +1018,7 @@ template <typename T, int VPT> __global__ __launch_bounds__(1024) void draw_fini
     for (int i = 0; i < kList; i++) z[i] = place_of(i) < listed ? list[place_of(i)].z : -HUGE_VALF;
     double w[kList];
 #pragma unroll
-    for (int i = 0; i < kList; i++) w[i] = draw_weight(z[i], max, c.inv_t);
+    for (int i = 0; i < kList; i++) w[i] = draw_weight(z[i], max, c.rate);
     if (draw_short_narrow<kThreads, kList>(z, w, at, max, min, c, shift, s.quick, &end)) {
 #pragma unroll
       for (int i = 0; i < kList; i++)
@@ -1002,7 +1038,7 @@ template <typename T, int VPT> __global__ __launch_bounds__(1024) void draw_fini
     unsigned long long *mass = s.quick.cmass, *place = s.quick.place;
     const double unit = ldexp(1.0, -shift);
     if (tid < listed) {
-      mass[tid] = draw_fixed(draw_weight(list[tid].z, max, c.inv_t), shift);
+      mass[tid] = draw_fixed(draw_weight(list[tid].z, max, c.rate), shift);
       place[tid] = draw_place(list[tid].z, list[tid].j);
     }
     if (tid == 0) s.quick.q[31] = 0;
@@ -1023,7 +1059,7 @@ template <typename T, int VPT> __global__ __launch_bounds__(1024) void draw_fini
   }
   // The kept mass of each unit
   auto weight_of = [&](float z, int j) {
-    const double w = z > -HUGE_VALF && end.kept(z, j) ? draw_weight(z, max, c.inv_t) : 0.0;
+    const double w = z > -HUGE_VALF && end.kept(z, j) ? draw_weight(z, max, c.rate) : 0.0;
     return w >= c.least ? w : 0.0;
   };
   double m[1] = {0.0};
@@ -1032,7 +1068,7 @@ template <typename T, int VPT> __global__ __launch_bounds__(1024) void draw_fini
       double v = 0.0;
       for (int i = 0; i < VPT; i++) {
         const int j = q * kUnit + i * kWave + lane;
-        if (j < n) v += weight_of((float)zp[j], j);
+        if (j < n) v += weight_of(draw_finite((float)zp[j]), j);
       }
       v = wave_sum(v);
       if (lane == 0) g.kept[row * g.units + q] = v;
@@ -1042,7 +1078,7 @@ template <typename T, int VPT> __global__ __launch_bounds__(1024) void draw_fini
   }
   if (tid < g.units) {
     if (kind == kRowPlain)
-      m[0] = part[tid].mass * draw_weight(part[tid].max, max, c.inv_t);
+      m[0] = part[tid].mass * draw_weight(part[tid].max, max, c.rate);
     else {
       m[0] = g.kept[row * g.units + tid];
       if (kind == kRowNucleus && !whole)
@@ -1064,7 +1100,7 @@ template <typename T, int VPT> __global__ __launch_bounds__(1024) void draw_fini
 #pragma unroll
   for (int i = 0; i < kIn; i++) {
     const int q = (wave * kIn + i) * kWave + lane, j = base + q;
-    w[i] = q < kUnit && j < n ? weight_of((float)zp[j], j) : 0.0;
+    w[i] = q < kUnit && j < n ? weight_of(draw_finite((float)zp[j]), j) : 0.0;
   }
   double ignored;
   const int place = draw_pick<kThreads, kIn, false>(w, aim, &ignored, &weight, &rest, s.quick.d);
@@ -1086,7 +1122,7 @@ template <typename T> __global__ __launch_bounds__(1024) void draw_huge_kernel(D
   for (int j = tid; j < n; j += kThreads) {
     const float z = (float)zp[j];
     nan |= z != z;
-    max = fmaxf(max, z);
+    max = fmaxf(max, draw_finite(z));
   }
   max = wave_max(max);
   const bool any = __any(nan);
@@ -1108,7 +1144,7 @@ template <typename T> __global__ __launch_bounds__(1024) void draw_huge_kernel(D
   }
   if (c.greedy) {
     for (int j = tid; j < n; j += kThreads)
-      if ((float)zp[j] == max) {
+      if (draw_finite((float)zp[j]) == max) {
         atomicMin(&first, (uint32_t)j);
         break;
       }
@@ -1118,8 +1154,8 @@ template <typename T> __global__ __launch_bounds__(1024) void draw_huge_kernel(D
   }
   const DrawEnd end = draw_whole<T, kThreads>(a, row, c, max, shift, s);
   auto weight_of = [&](int j) {
-    const float z = (float)zp[j];
-    const double w = z > -HUGE_VALF && end.kept(z, j) ? draw_weight(z, max, c.inv_t) : 0.0;
+    const float z = draw_finite((float)zp[j]);
+    const double w = z > -HUGE_VALF && end.kept(z, j) ? draw_weight(z, max, c.rate) : 0.0;
     return w >= c.least ? w : 0.0;
   };
   // Runs of columns, one a wave; then the run in which the kept mass exceeds u of it is cut into runs again.

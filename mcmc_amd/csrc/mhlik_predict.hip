@@ -211,7 +211,11 @@ template <typename T, int VEC, int VPT> void draw_long(const DrawArgs &a, const 
 {
   const dim3 grid((unsigned)(a.rows * g.groups));
   hipLaunchKernelGGL((draw_top_kernel<T, VEC, VPT>), grid, dim3(kBlock), 0, stream, a, g, (int)histo);
-  if (histo) hipLaunchKernelGGL((draw_histo_kernel<T, VEC, VPT>), grid, dim3(kBlock), 0, stream, a, g, shift);
+  if (histo) { // a workgroup's histogram is added to the row's at the end: no more workgroups than fill the chip four times
+    int groups = g.groups;
+    while (groups > 1 && a.rows * groups > 1024) groups = (groups + 1) / 2;
+    hipLaunchKernelGGL((draw_histo_kernel<T, VEC, VPT>), dim3((unsigned)(a.rows * groups)), dim3(kBlock), 0, stream, a, g, groups, shift);
+  }
   if (collect) hipLaunchKernelGGL((draw_collect_kernel<T, VEC, VPT>), grid, dim3(kBlock), 0, stream, a, g, shift);
   hipLaunchKernelGGL((draw_finish_kernel<T, VPT>), dim3((unsigned)a.rows), dim3(1024), 0, stream, a, g, shift);
 }
@@ -239,15 +243,10 @@ template <typename T> int draw_launch(const DrawArgs &a, void *workspace, size_t
     const bool histo = a.top_k || a.top_p || (a.top_k_all > 0 && a.top_k_all < a.n) || a.top_p_all < 1.0;
     const bool collect = histo || a.min_p || a.min_p_all > 0.0;
     constexpr int kVec = 16 / sizeof(T);
-    const bool vec = aligned16(a.z) && (a.rows == 1 || a.stride * (int64_t)sizeof(T) % 16 == 0);
-    if (p.vpt == 8 && vec)
+    if (p.vpt == 8)
       draw_long<T, kVec, 8>(a, p.space, shift, histo, collect, stream);
-    else if (p.vpt == 8)
-      draw_long<T, 1, 8>(a, p.space, shift, histo, collect, stream);
-    else if (vec)
-      draw_long<T, kVec, kLongVpt>(a, p.space, shift, histo, collect, stream);
     else
-      draw_long<T, 1, kLongVpt>(a, p.space, shift, histo, collect, stream);
+      draw_long<T, kVec, kLongVpt>(a, p.space, shift, histo, collect, stream);
   }
   PCHK(hipGetLastError());
   return MHLIK_OK;
