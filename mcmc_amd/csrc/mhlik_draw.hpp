@@ -397,9 +397,10 @@ __device__ void draw_narrow(DrawRow<T> &r, DrawShared &s, int shift, uint32_t k,
 
 // ------------------------------------------------ rows that fit a workgroup
 //
-// The values stay in registers, 64 consecutive columns to a wave's register.  One histogram by distance from the largest
-// (counts and masses) gives the bin in which a border falls; the few values of that bin go to LDS and each finds its
-// rank, and the mass before it, by comparing with all others.
+// The values stay in registers, 64 consecutive columns to a wave's register.  A histogram by distance from the largest
+// gives the bin in which the border falls; the few values of that bin go to LDS and each finds its rank, and the mass
+// before it, by comparing with all others.  Top-k first, over counts (32-bit atomics: of all values), then top-p, over
+// masses (64-bit ones: only of what top-k left).
 
 template <int THREADS> struct ShortShared {
   static constexpr int kCap = THREADS; // values of a border's bin
@@ -414,170 +415,152 @@ template <int THREADS> struct ShortShared {
   uint32_t i[32];
 };
 
-// Narrows the kept prefix.  z: -inf where there is nothing; column j of z[i] from at(i); weight: of z[i].  Returns false if a border's
-// bin holds more values than there is room for.
-template <int THREADS, int VPT, typename AT>
-__device__ bool draw_short_narrow(const float (&z)[VPT], const double (&weight)[VPT], AT at, float max, float min, const DrawChoice &c,
-                                  int shift, ShortShared<THREADS> &s, DrawEnd *end)
+// The sum before this thread's bins, from its own `mine`; *all: of all bins.  One barrier; lds is free after the next.
+template <int THREADS, typename V> __device__ __forceinline__ V draw_before(V mine, V *all, V *lds)
 {
-  constexpr int kWaves = THREADS / kWave, kShortBins = ShortShared<THREADS>::kBins, kRun = kShortBins / THREADS;
-  const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
-  const DrawBin<kShortBins> bin(max, min, c.temp);
-  const bool by_mass = c.share < 1.0;
+  constexpr int kWaves = THREADS / kWave;
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  const V in = wave_running(mine);
+  if (lane == kWave - 1) lds[wave] = in;
+  __syncthreads();
+  V before = in - mine, sum = 0;
+#pragma unroll
+  for (int w = 0; w < kWaves; w++) {
+    const V v = lds[w];
+    if (w < wave) before += v;
+    sum += v;
+  }
+  *all = sum;
+  return before;
+}
+
+// The place of the k-th of the values above -inf; unchanged if there are no more than k.  False: no room.
+template <int THREADS, int VPT, int BINS, typename AT>
+__device__ bool draw_by_count(const float (&z)[VPT], AT at, const DrawBin<BINS> &bin, uint32_t k, ShortShared<THREADS> &s, DrawEnd *end)
+{
+  constexpr int kRun = BINS / THREADS;
+  const int tid = threadIdx.x;
+#pragma unroll
+  for (int i = 0; i < kRun; i++) s.count[tid + i * THREADS] = 0;
+  if (tid == 0) s.i[30] = 0;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < VPT; i++)
+    if (z[i] > -HUGE_VALF) atomicAdd(&s.count[bin.of(z[i])], 1u);
+  __syncthreads();
+  uint32_t here[kRun], mine = 0, all;
+#pragma unroll
+  for (int i = 0; i < kRun; i++) mine += here[i] = s.count[tid * kRun + i];
+  uint32_t n = draw_before<THREADS>(mine, &all, s.i);
+  if (all <= k) return true;
+#pragma unroll
+  for (int i = 0; i < kRun; i++) {
+    if (n < k && n + here[i] >= k) {
+      s.i[31] = tid * kRun + i;
+      s.i[29] = n;
+    }
+    n += here[i];
+  }
+  __syncthreads();
+  const int border = (int)s.i[31];
+#pragma unroll
+  for (int i = 0; i < VPT; i++)
+    if (z[i] > -HUGE_VALF && bin.of(z[i]) == border) {
+      const uint32_t q = atomicAdd(&s.i[30], 1u);
+      if (q < ShortShared<THREADS>::kCap) s.place[q] = draw_place(z[i], at(i));
+    }
+  __syncthreads();
+  const int m = (int)s.i[30];
+  if (m > ShortShared<THREADS>::kCap) return false;
+  if (tid < m) {
+    const unsigned long long own = s.place[tid];
+    uint32_t rank = s.i[29];
+    for (int q = 0; q < m; q++) rank += s.place[q] < own;
+    if (rank == k - 1) s.q[31] = own;
+  }
+  __syncthreads();
+  end->place = s.q[31];
+  return true;
+}
+
+// Of the values up to end->place, the place of the last before which (with `base` before them all) less than the target
+// lies; share: the target is this share of their mass.  False: no room.
+template <int THREADS, int VPT, int BINS, typename AT>
+__device__ bool draw_by_mass(const float (&z)[VPT], const double (&weight)[VPT], AT at, const DrawBin<BINS> &bin, unsigned long long base,
+                             double share, double target, int shift, ShortShared<THREADS> &s, DrawEnd *end)
+{
+  constexpr int kRun = BINS / THREADS;
+  const int tid = threadIdx.x;
   const double unit = ldexp(1.0, -shift);
-  for (int b = tid; b < kShortBins; b += THREADS) {
-    s.count[b] = 0;
-    s.mass[b] = 0;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kRun; i++) s.mass[tid + i * THREADS] = 0;
+  if (tid == 0) {
+    s.i[30] = 0;
+    s.i[31] = BINS;
   }
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < VPT; i++)
-    if (z[i] > -HUGE_VALF) {
-      const int b = bin.of(z[i]);
-      atomicAdd(&s.count[b], 1u);
-      if (by_mass) {
-        const unsigned long long m = draw_fixed(weight[i], shift);
-        if (m) atomicAdd(&s.mass[b], m);
-      }
+    if (weight[i] > 0.0 && end->kept(z[i], at(i))) {
+      const unsigned long long m = draw_fixed(weight[i], shift);
+      if (m) atomicAdd(&s.mass[bin.of(z[i])], m);
     }
   __syncthreads();
-  // sums before each bin; a thread has kRun bins
-  uint32_t cn = 0;
-  unsigned long long cm = 0;
+  unsigned long long here[kRun], mine = 0, all;
+#pragma unroll
+  for (int i = 0; i < kRun; i++) mine += here[i] = s.mass[tid * kRun + i];
+  unsigned long long before = base + draw_before<THREADS>(mine, &all, s.q);
+  if (share >= 0.0) target = share * ((double)all * unit);
 #pragma unroll
   for (int i = 0; i < kRun; i++) {
-    cn += s.count[tid * kRun + i];
-    cm += s.mass[tid * kRun + i];
+    if (here[i] && ((double)before * unit < target || before == 0) && (double)(before + here[i]) * unit >= target) {
+      s.i[31] = tid * kRun + i; // one bin at most: the sums grow
+      s.q[29] = before;
+    }
+    before += here[i];
   }
-  uint32_t in = wave_running(cn);
-  unsigned long long im = wave_running(cm);
-  if (lane == kWave - 1) {
-    s.i[wave] = in;
-    s.q[wave] = im;
-  }
-  if (tid == 0) {
-    s.i[31] = kShortBins; // the bin of the top-k border
-    s.i[30] = 0;          // values gathered
+  if (tid == 0) s.q[31] = 0;
+  __syncthreads();
+  const int border = (int)s.i[31];
+  if (border == BINS) return true; // what is here ends before the target: all of it
+#pragma unroll
+  for (int i = 0; i < VPT; i++)
+    if (weight[i] > 0.0 && end->kept(z[i], at(i)) && bin.of(z[i]) == border) {
+      const uint32_t q = atomicAdd(&s.i[30], 1u);
+      if (q < ShortShared<THREADS>::kCap) {
+        s.place[q] = draw_place(z[i], at(i));
+        s.cmass[q] = draw_fixed(weight[i], shift);
+      }
+    }
+  __syncthreads();
+  const int m = (int)s.i[30];
+  if (m > ShortShared<THREADS>::kCap) return false;
+  if (tid < m) {
+    const unsigned long long own = s.place[tid];
+    unsigned long long b = s.q[29];
+    uint32_t rank = 0;
+    for (int q = 0; q < m; q++) {
+      const bool earlier = s.place[q] < own;
+      b += earlier ? s.cmass[q] : 0;
+      rank += earlier;
+    }
+    if ((double)b * unit < target || (s.q[29] == 0 && rank == 0)) atomicMax(&s.q[31], own);
   }
   __syncthreads();
-  uint32_t some = 0;
-  unsigned long long all = 0;
-#pragma unroll
-  for (int w = 0; w < kWaves; w++) {
-    if (w < wave) {
-      in += s.i[w];
-      im += s.q[w];
-    }
-    some += s.i[w];
-    all += s.q[w];
-  }
-  const bool by_count = c.k > 0 && (uint32_t)c.k < some;
-  unsigned long long place = ~0ull; // the last kept
-  int gathered = -1;
-  if (by_count) {
-    uint32_t n = in - cn;
-    unsigned long long m = im - cm;
-    for (int i = 0; i < kRun; i++) {
-      const uint32_t here = s.count[tid * kRun + i];
-      if (n < (uint32_t)c.k && n + here >= (uint32_t)c.k) {
-        s.i[31] = tid * kRun + i;
-        s.i[29] = n;
-        s.q[29] = m;
-      }
-      n += here;
-      m += s.mass[tid * kRun + i];
-    }
-    __syncthreads();
-    gathered = (int)s.i[31];
-  }
-  // Bring the values of bin `gathered` to LDS; *m: how many
-  auto gather = [&](int which) {
-#pragma unroll
-    for (int i = 0; i < VPT; i++)
-      if (z[i] > -HUGE_VALF && bin.of(z[i]) == which) {
-        const uint32_t q = atomicAdd(&s.i[30], 1u);
-        if (q < ShortShared<THREADS>::kCap) {
-          s.place[q] = draw_place(z[i], at(i));
-          s.cmass[q] = by_mass ? draw_fixed(weight[i], shift) : 0;
-        }
-      }
-    __syncthreads();
-    return (int)s.i[30];
-  };
-  int m = 0;
-  unsigned long long before = 0; // of this thread's value, in its bin
-  uint32_t rank = 0;
-  auto order = [&]() {
-    before = 0;
-    rank = 0;
-    if (tid < m) {
-      const unsigned long long mine = s.place[tid];
-      for (int q = 0; q < m; q++)
-        if (s.place[q] < mine) {
-          rank++;
-          before += s.cmass[q];
-        }
-    }
-  };
-  if (by_count) {
-    m = gather(gathered);
-    if (m > ShortShared<THREADS>::kCap) return false;
-    order();
-    if (tid < m && s.i[29] + rank == (uint32_t)c.k - 1) {
-      s.q[31] = s.place[tid];
-      s.q[30] = s.q[29] + before + s.cmass[tid];
-    }
-    __syncthreads();
-    place = s.q[31];
-    all = s.q[30];
-  }
-  if (by_mass) {
-    const double target = c.share * ((double)all * unit);
-    // the last value before which less than the target lies
-    __syncthreads();
-    if (tid == 0) {
-      s.i[31] = kShortBins;
-      s.q[31] = 0;
-    }
-    __syncthreads();
-    uint32_t n = in - cn;
-    unsigned long long below = im - cm;
-    for (int i = 0; i < kRun; i++) {
-      const uint32_t here = s.count[tid * kRun + i];
-      const unsigned long long hm = s.mass[tid * kRun + i];
-      const bool first = n == 0;
-      if (here && ((double)below * unit < target || first) && (double)(below + hm) * unit >= target) {
-        atomicMin(&s.i[31], (uint32_t)(tid * kRun + i));
-      }
-      n += here;
-      below += hm;
-    }
-    __syncthreads();
-    int which = (int)s.i[31];
-    if (by_count && which > gathered) which = gathered;
-    // what lies before that bin
-    if (which / kRun == tid) {
-      unsigned long long b = im - cm;
-      for (int i = 0; i < which % kRun; i++) b += s.mass[tid * kRun + i];
-      s.q[29] = b;
-    }
-    if (tid == 0 && which != gathered) s.i[30] = 0;
-    __syncthreads();
-    const unsigned long long base = s.q[29];
-    if (which != gathered) {
-      m = gather(which);
-      if (m > ShortShared<THREADS>::kCap) return false;
-      order();
-    }
-    if (tid < m) {
-      const unsigned long long mine = s.place[tid];
-      if (mine <= place && ((double)(base + before) * unit < target || (base == 0 && rank == 0))) atomicMax(&s.q[31], mine);
-    }
-    __syncthreads();
-    place = s.q[31];
-  }
-  end->place = place;
+  end->place = s.q[31];
   return true;
+}
+
+// Narrows the kept prefix by the row's top-k and top-p.  z: -inf where there is nothing; column j of z[i] from at(i);
+// weight: of z[i].  False if a border's bin holds more values than there is room for.
+template <int THREADS, int VPT, typename AT>
+__device__ bool draw_short_narrow(const float (&z)[VPT], const double (&weight)[VPT], AT at, float max, float min, const DrawChoice &c,
+                                  int shift, ShortShared<THREADS> &s, DrawEnd *end)
+{
+  const DrawBin<ShortShared<THREADS>::kBins> bin(max, min, c.temp);
+  if (c.k && !draw_by_count<THREADS, VPT>(z, at, bin, (uint32_t)c.k, s, end)) return false;
+  return c.share >= 1.0 || draw_by_mass<THREADS, VPT>(z, weight, at, bin, 0, c.share, 0.0, shift, s, end);
 }
 
 // What the kernels that finish a row keep in LDS: one of the two at a time.
@@ -824,6 +807,10 @@ __global__ __launch_bounds__(kBlock) void draw_histo_kernel(DrawArgs a, LongSpac
   __shared__ unsigned long long bins[kLongBins];
   const int64_t row = blockIdx.x / groups;
   const int group = blockIdx.x % groups, wave = threadIdx.x / kWave;
+  const T *zp = (const T *)a.z + row * a.stride;
+  int unit = group * 4 + wave;
+  float z[VPT]; // on their way before it is known what the row needs
+  if (unit < g.units) draw_load<T, VEC, VPT>(zp, (int)a.n, unit * VPT * kWave, z);
   float max, min;
   bool nan;
   draw_row_range(g.part + row * g.units, g.units, &max, &min, &nan);
@@ -833,15 +820,15 @@ __global__ __launch_bounds__(kBlock) void draw_histo_kernel(DrawArgs a, LongSpac
   for (int b = threadIdx.x; b < kLongBins; b += kBlock) bins[b] = 0;
   __syncthreads();
   const DrawBin<kLongBins> bin(max, min, c.temp);
-  for (int unit = group * 4 + wave; unit < g.units; unit += groups * 4) {
-    float z[VPT];
-    draw_load<T, VEC, VPT>((const T *)a.z + row * a.stride, (int)a.n, unit * VPT * kWave, z);
+  while (unit < g.units) {
 #pragma unroll
     for (int i = 0; i < VPT; i++)
       if (z[i] > -HUGE_VALF) {
         const unsigned long long m = kind == kRowList ? 1 : draw_fixed(draw_weight(z[i], max, c.rate), shift);
         if (m) atomicAdd(&bins[bin.of(z[i])], m);
       }
+    unit += groups * 4;
+    if (unit < g.units) draw_load<T, VEC, VPT>(zp, (int)a.n, unit * VPT * kWave, z);
   }
   __syncthreads();
   for (int b = threadIdx.x; b < kLongBins; b += kBlock)
@@ -855,6 +842,10 @@ __global__ __launch_bounds__(kBlock) void draw_collect_kernel(DrawArgs a, LongSp
   __shared__ LongCell cell;
   const int64_t row = blockIdx.x / g.groups;
   const int tid = threadIdx.x, group = blockIdx.x % g.groups, wave = tid / kWave, lane = tid % kWave;
+  constexpr int kUnit = VPT * kWave;
+  const int u = group * 4 + wave;
+  float z[VPT];
+  if (u < g.units) draw_load<T, VEC, VPT>((const T *)a.z + row * a.stride, (int)a.n, u * kUnit, z);
   float max, min;
   bool nan;
   draw_row_range(g.part + row * g.units, g.units, &max, &min, &nan);
@@ -897,11 +888,7 @@ __global__ __launch_bounds__(kBlock) void draw_collect_kernel(DrawArgs a, LongSp
     too_long = cell.too_long;
     if (group == 0 && tid == 0) g.cell[row] = cell;
   }
-  const int u = group * 4 + wave;
   if (u >= g.units || too_long) return;
-  constexpr int kUnit = VPT * kWave;
-  float z[VPT];
-  draw_load<T, VEC, VPT>((const T *)a.z + row * a.stride, (int)a.n, u * kUnit, z);
   const DrawBin<kLongBins> bin(max, min, c.temp);
   double kept = 0.0;
   int n = 0;
@@ -995,7 +982,7 @@ template <typename T, int VPT> __global__ __launch_bounds__(1024) void draw_fini
       }
       if (tid < g.units) from[tid] = in - mine;
       __syncthreads();
-      whole = listed > (kind == kRowList ? kLongList : kThreads);
+      whole = listed > kLongList;
     }
     if (!whole) { // each thread finds the unit of its entry: the last one that begins at or before it
       for (int i = tid; i < listed; i += kThreads) {
@@ -1009,17 +996,18 @@ template <typename T, int VPT> __global__ __launch_bounds__(1024) void draw_fini
       __syncthreads();
     }
   }
-  if (kind == kRowList && !whole) {
+  if (kind >= kRowList && !whole) {
     constexpr int kList = kLongList / kThreads;
     float z[kList];
+    double w[kList];
     auto place_of = [&](int i) { return (wave * kList + i) * kWave + lane; };
     auto at = [&](int i) { return list[place_of(i)].j; };
 #pragma unroll
-    for (int i = 0; i < kList; i++) z[i] = place_of(i) < listed ? list[place_of(i)].z : -HUGE_VALF;
-    double w[kList];
-#pragma unroll
-    for (int i = 0; i < kList; i++) w[i] = draw_weight(z[i], max, c.rate);
-    if (draw_short_narrow<kThreads, kList>(z, w, at, max, min, c, shift, s.quick, &end)) {
+    for (int i = 0; i < kList; i++) {
+      z[i] = place_of(i) < listed ? list[place_of(i)].z : -HUGE_VALF;
+      w[i] = draw_weight(z[i], max, c.rate);
+    }
+    if (kind == kRowList && draw_short_narrow<kThreads, kList>(z, w, at, max, min, c, shift, s.quick, &end)) {
 #pragma unroll
       for (int i = 0; i < kList; i++)
         if (!end.kept(z[i], at(i)) || w[i] < c.least) w[i] = 0.0;
@@ -1029,34 +1017,34 @@ template <typename T, int VPT> __global__ __launch_bounds__(1024) void draw_fini
       if (place >= 0) draw_answer(a, row, list[place].j, log(weight / total));
       return;
     }
-    whole = true;
+    if (kind == kRowNucleus) { // the border lies among the listed, which are one bin of the row: bins within it
+      float top = -HUGE_VALF, low = HUGE_VALF;
+#pragma unroll
+      for (int i = 0; i < kList; i++) {
+        top = fmaxf(top, z[i]);
+        if (z[i] > -HUGE_VALF) low = fminf(low, z[i]);
+      }
+      top = wave_max(top);
+      low = wave_min(low);
+      if (lane == 0) {
+        s.quick.f[wave] = top;
+        s.quick.g[wave] = low;
+      }
+      __syncthreads();
+#pragma unroll
+      for (int q = 0; q < kThreads / kWave; q++) {
+        top = fmaxf(top, s.quick.f[q]);
+        low = fminf(low, s.quick.g[q]);
+      }
+      const DrawBin<ShortShared<kThreads>::kBins> bin(top, low, HUGE_VAL);
+      whole = !draw_by_mass<kThreads, kList>(z, w, at, bin, cell.above, -1.0, cell.target, shift, s.quick, &end);
+      if (whole) end.place = ~0ull;
+    } else
+      whole = true;
   }
   const T *zp = (const T *)a.z + row * a.stride;
   const int n = (int)a.n;
   if (whole) end = draw_whole<T, kThreads>(a, row, c, max, shift, s.whole);
-  if (kind == kRowNucleus && !whole) { // the border among the listed
-    unsigned long long *mass = s.quick.cmass, *place = s.quick.place;
-    const double unit = ldexp(1.0, -shift);
-    if (tid < listed) {
-      mass[tid] = draw_fixed(draw_weight(list[tid].z, max, c.rate), shift);
-      place[tid] = draw_place(list[tid].z, list[tid].j);
-    }
-    if (tid == 0) s.quick.q[31] = 0;
-    __syncthreads();
-    if (tid < listed) {
-      const unsigned long long mine = place[tid];
-      unsigned long long before = cell.above;
-      int rank = 0;
-      for (int q = 0; q < listed; q++)
-        if (place[q] < mine) {
-          before += mass[q];
-          rank++;
-        }
-      if ((double)before * unit < cell.target || (cell.above == 0 && rank == 0)) atomicMax(&s.quick.q[31], mine);
-    }
-    __syncthreads();
-    end.place = s.quick.q[31];
-  }
   // The kept mass of each unit
   auto weight_of = [&](float z, int j) {
     const double w = z > -HUGE_VALF && end.kept(z, j) ? draw_weight(z, max, c.rate) : 0.0;
