@@ -158,7 +158,7 @@ template <int THREADS, int VPT, bool IS_SHARE>
 __device__ int draw_pick(const double (&w)[VPT], double aim, double *total, double *weight, double *rest, double *lds /* [THREADS / 64] */)
 {
   constexpr int kWaves = THREADS / kWave;
-  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   double m = 0.0;
 #pragma unroll
   for (int i = 0; i < VPT; i++) m += w[i];
@@ -166,43 +166,33 @@ __device__ int draw_pick(const double (&w)[VPT], double aim, double *total, doub
   __syncthreads();
   if (lane == 0) lds[wave] = m;
   __syncthreads();
+  // the first wave that exceeds the aim; if rounding leaves none, the last with any mass
+  const double of = lane < kWaves ? lds[lane] : 0.0, upto = wave_running(of);
   if (IS_SHARE) {
-    double t = 0.0;
-#pragma unroll
-    for (int q = 0; q < kWaves; q++) t += lds[q];
-    *total = t;
-    aim *= t;
+    *total = wave_last(upto);
+    aim *= *total;
   }
-  int pick = -1; // the first wave that exceeds the aim; if rounding leaves none, the last with any mass
-  double before = 0.0, sum = 0.0;
-  for (int q = 0; q < kWaves; q++) {
-    const double v = lds[q];
-    if (v > 0.0) {
-      pick = q;
-      before = sum;
-      if (sum + v > aim) break;
-    }
-    sum += v;
-  }
+  const unsigned long long passed = __ballot(of > 0.0 && upto > aim), any = __ballot(of > 0.0);
+  const int pick = passed ? __ffsll(passed) - 1 : 63 - __clzll((long long)any);
+  const double before = pick > 0 ? wave_lane(upto, pick - 1) : 0.0;
   int place = -1;
   if (wave == pick) {
     aim -= before;
-    sum = before = 0.0;
     int at = -1;
-    double mine = 0.0;
+    double sum = 0.0, done_before = 0.0, mine = 0.0;
     bool done = false;
 #pragma unroll
     for (int i = 0; i < VPT; i++) { // the same for the runs of 64
       const double v = wave_sum(w[i]);
       if (!done && v > 0.0) {
         at = i;
-        before = sum;
+        done_before = sum;
         mine = w[i];
         done = sum + v > aim;
       }
       sum += v;
     }
-    aim -= before;
+    aim -= done_before;
     const double run = wave_running(mine);
     const unsigned long long over = __ballot(mine > 0.0 && run > aim), some = __ballot(mine > 0.0);
     const int who = over ? __ffsll(over) - 1 : 63 - __clzll((long long)some);
@@ -215,13 +205,26 @@ __device__ int draw_pick(const double (&w)[VPT], double aim, double *total, doub
   return place;
 }
 
+// The sum before this thread's bins, from its own `mine`; *all: of all bins.  One barrier; lds is free after the next.
+template <int THREADS, typename V> __device__ __forceinline__ V draw_before(V mine, V *all, V *lds)
+{
+  constexpr int kWaves = THREADS / kWave;
+  const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const V in = wave_running(mine);
+  if (lane == kWave - 1) lds[wave] = in;
+  __syncthreads();
+  const V upto = wave_running(lane < kWaves ? lds[lane] : (V)0);
+  *all = wave_last(upto);
+  return in - mine + (wave > 0 ? wave_lane(upto, wave - 1) : (V)0);
+}
+
 // ---------------------------------------------------- whole rows, any data
 //
-// The key of the border is found eleven bits at a time, each time from a histogram over the whole row.  It needs nothing
+// The key of the border is found eight bits at a time, each time from a histogram over the whole row.  It needs nothing
 // of the data and serves the rows that the quick ways below hand back: more equal (or nearly equal) values at a border
 // than they have places for, a top-k of thousands.
 
-constexpr int kDrawBins = 2048;
+constexpr int kDrawBins = 256;
 
 // What a workgroup shares.
 struct DrawShared {
@@ -245,8 +248,8 @@ template <typename T> struct DrawRow {
 };
 
 // The prefix of the kept order that is needed for `k` values (BY_MASS false) or for `share` of the kept mass (true):
-// key and column are narrowed.  The key is found eleven bits at a time from a histogram of the values that share the
-// bits found so far.
+// key and column are narrowed.  The key is found eight bits at a time from a histogram of the values that share the bits
+// found so far.
 template <typename T, int THREADS, bool BY_MASS>
 __device__ void draw_narrow(DrawRow<T> &r, DrawShared &s, int shift, uint32_t k, double share)
 {
@@ -256,8 +259,8 @@ __device__ void draw_narrow(DrawRow<T> &r, DrawShared &s, int shift, uint32_t k,
   unsigned long long above_m = 0;
   double target = 0.0;
   uint32_t equal = 0;
-  for (int level = 0; level < 3; level++) {
-    const int low = level == 0 ? 21 : level == 1 ? 10 : 0, bits = level == 2 ? 10 : 11, high = low + bits;
+  for (int level = 0; level < 4; level++) {
+    const int low = 24 - 8 * level, high = low + 8;
     for (int b = tid; b < kDrawBins; b += THREADS) {
       s.count[b] = 0;
       if (BY_MASS) s.mass[b] = 0;
@@ -268,7 +271,7 @@ __device__ void draw_narrow(DrawRow<T> &r, DrawShared &s, int shift, uint32_t k,
       const uint32_t key = draw_key(z);
       if (level && key >> high != prefix) continue;
       if (!r.kept(key, j)) continue;
-      const uint32_t bin = (key >> low) & ((1u << bits) - 1);
+      const uint32_t bin = (key >> low) & 255u;
       atomicAdd(&s.count[bin], 1u);
       if (BY_MASS) {
         const unsigned long long m = (unsigned long long)rint(ldexp(draw_weight(z, r.max, r.rate), shift));
@@ -276,74 +279,55 @@ __device__ void draw_narrow(DrawRow<T> &r, DrawShared &s, int shift, uint32_t k,
       }
     }
     __syncthreads();
-    // sums from the top bin down; each thread takes a run of bins
-    constexpr int kRun = kDrawBins / THREADS;
-    uint32_t cn = 0;
-    unsigned long long cm = 0;
-    const int top = kDrawBins - 1 - tid * kRun;
+    // sums from the top bin down; a thread has kRun bins, or none
+    constexpr int kRun = THREADS >= kDrawBins ? 1 : kDrawBins / THREADS;
+    const bool has = tid * kRun < kDrawBins;
+    uint32_t cn[kRun], n = 0, some;
+    unsigned long long cm[kRun], m = 0, all;
+#pragma unroll
     for (int i = 0; i < kRun; i++) {
-      cn += s.count[top - i];
-      if (BY_MASS) cm += s.mass[top - i];
+      n += cn[i] = has ? s.count[kDrawBins - 1 - tid * kRun - i] : 0;
+      m += cm[i] = has && BY_MASS ? s.mass[kDrawBins - 1 - tid * kRun - i] : 0;
     }
-    const uint32_t in = wave_running(cn);
-    const unsigned long long im = wave_running(cm);
-    const int lane = tid % kWave;
-    if (lane == kWave - 1) {
-      s.i[tid / kWave] = in;
-      s.q[tid / kWave] = im;
-    }
-    __syncthreads();
-    uint32_t bn = above_n;
-    unsigned long long bm = above_m, all = 0;
-    for (int w = 0; w < THREADS / kWave; w++) {
-      if (w < tid / kWave) {
-        bn += s.i[w];
-        bm += s.q[w];
-      }
-      all += s.q[w];
-    }
+    n = above_n + draw_before<THREADS>(n, &some, s.i);
+    m = above_m + draw_before<THREADS>(m, &all, s.q);
     if (BY_MASS && level == 0) target = share * ((double)all * unit);
-    // the first bin, from the top, that reaches the aim; the mass may miss it by rounding: then the lowest bin in use
-    __syncthreads();
     if (tid == 0) {
-      s.i[31] = 0xffffffffu;
-      s.i[30] = 0xffffffffu;
+      s.i[31] = 0;
+      s.i[30] = 0;
     }
     __syncthreads();
-    uint32_t n = bn + in - cn;
-    unsigned long long m = bm + im - cm;
+    // the first bin, from the top, that reaches the aim; the mass may miss it by rounding: then the lowest bin in use
+#pragma unroll
     for (int i = 0; i < kRun; i++) {
-      const uint32_t c = s.count[top - i];
-      const unsigned long long w = BY_MASS ? s.mass[top - i] : 0;
-      if (c) {
-        atomicMin(&s.i[30], (uint32_t)(top - i));
-        const bool reach = BY_MASS ? (double)(m + w) * unit >= target : n + c >= k;
+      if (cn[i]) {
+        const uint32_t bin = kDrawBins - 1 - tid * kRun - i;
+        atomicMax(&s.i[30], kDrawBins - bin);
+        const bool reach = BY_MASS ? (double)(m + cm[i]) * unit >= target : n + cn[i] >= k;
         const bool before = BY_MASS ? (double)m * unit >= target && n > 0 : n >= k;
-        if (reach && !before) s.i[31] = (uint32_t)(top - i);
+        if (reach && !before) s.i[31] = kDrawBins - bin;
       }
-      n += c;
-      m += w;
+      n += cn[i];
+      m += cm[i];
     }
     __syncthreads();
-    const uint32_t bin = s.i[31] != 0xffffffffu ? s.i[31] : s.i[30];
+    const uint32_t bin = kDrawBins - (s.i[31] ? s.i[31] : s.i[30]);
     // what lies above that bin
-    __syncthreads();
-    n = bn + in - cn;
-    m = bm + im - cm;
-    for (int i = 0; i < kRun; i++) {
-      if ((uint32_t)(top - i) == bin) {
+#pragma unroll
+    for (int i = kRun - 1; i >= 0; i--) {
+      n -= cn[i];
+      m -= cm[i];
+      if (has && kDrawBins - 1 - tid * kRun - i == (int)bin) {
         s.i[29] = n;
         s.q[29] = m;
-        s.i[28] = s.count[bin];
+        s.i[28] = cn[i];
       }
-      n += s.count[top - i];
-      m += BY_MASS ? s.mass[top - i] : 0;
     }
     __syncthreads();
     above_n = s.i[29];
     above_m = s.q[29];
     equal = s.i[28];
-    prefix = prefix << bits | bin;
+    prefix = prefix << 8 | bin;
     __syncthreads();
   }
   // `prefix` is the key now; of its `equal` columns the first `take` are needed
@@ -403,8 +387,8 @@ __device__ void draw_narrow(DrawRow<T> &r, DrawShared &s, int shift, uint32_t k,
 // masses (64-bit ones: only of what top-k left).
 
 template <int THREADS> struct ShortShared {
-  static constexpr int kCap = THREADS; // values of a border's bin
-  static constexpr int kBins = THREADS == 1024 ? 1024 : 512;
+  static constexpr int kBins = THREADS < 256 ? 256 : THREADS;          // one a thread, or four
+  static constexpr int kCap = THREADS < 256 ? 128 : THREADS;           // values of a border's bin
   unsigned long long mass[kBins];
   uint32_t count[kBins];
   unsigned long long place[kCap];
@@ -414,25 +398,6 @@ template <int THREADS> struct ShortShared {
   float f[32], g[32];
   uint32_t i[32];
 };
-
-// The sum before this thread's bins, from its own `mine`; *all: of all bins.  One barrier; lds is free after the next.
-template <int THREADS, typename V> __device__ __forceinline__ V draw_before(V mine, V *all, V *lds)
-{
-  constexpr int kWaves = THREADS / kWave;
-  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-  const V in = wave_running(mine);
-  if (lane == kWave - 1) lds[wave] = in;
-  __syncthreads();
-  V before = in - mine, sum = 0;
-#pragma unroll
-  for (int w = 0; w < kWaves; w++) {
-    const V v = lds[w];
-    if (w < wave) before += v;
-    sum += v;
-  }
-  *all = sum;
-  return before;
-}
 
 // The place of the k-th of the values above -inf; unchanged if there are no more than k.  False: no room.
 template <int THREADS, int VPT, int BINS, typename AT>
@@ -472,8 +437,8 @@ __device__ bool draw_by_count(const float (&z)[VPT], AT at, const DrawBin<BINS> 
   __syncthreads();
   const int m = (int)s.i[30];
   if (m > ShortShared<THREADS>::kCap) return false;
-  if (tid < m) {
-    const unsigned long long own = s.place[tid];
+  for (int c = tid; c < m; c += THREADS) {
+    const unsigned long long own = s.place[c];
     uint32_t rank = s.i[29];
     for (int q = 0; q < m; q++) rank += s.place[q] < own;
     if (rank == k - 1) s.q[31] = own;
@@ -536,8 +501,8 @@ __device__ bool draw_by_mass(const float (&z)[VPT], const double (&weight)[VPT],
   __syncthreads();
   const int m = (int)s.i[30];
   if (m > ShortShared<THREADS>::kCap) return false;
-  if (tid < m) {
-    const unsigned long long own = s.place[tid];
+  for (int c = tid; c < m; c += THREADS) {
+    const unsigned long long own = s.place[c];
     unsigned long long b = s.q[29];
     uint32_t rank = 0;
     for (int q = 0; q < m; q++) {

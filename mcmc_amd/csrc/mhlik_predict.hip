@@ -228,11 +228,23 @@ template <typename T> int draw_launch(const DrawArgs &a, void *workspace, size_t
   if (p.bytes && (!aligned16(workspace) || !workspace || workspace_bytes < p.bytes))
     return fail_no_ctx(MHLIK_EINVAL, "workspace: %zu bytes at a multiple of 16 are needed (%zu given)", p.bytes, workspace_bytes);
   if (p.short_rows) {
+    // Many rows: few waves a row, since a wave's own cost (scans, the border) adds up (top-k, top-p and min-p, 4096 rows:
+    // of 2000, 4 waves 39 us, 8 waves 47; of 400, 1 wave 14 us, 4 waves 20).  Few rows: as many waves as there is work
+    // for, which shortens a row's chain of steps (1 row of 1000: 8 waves 7.1 us, 4 waves 8.4).
     const dim3 grid((unsigned)a.rows);
-    if (a.n <= 512)
+    const bool many = a.rows >= 512;
+    if (many && a.n <= 128)
+      hipLaunchKernelGGL((draw_short_kernel<T, 64, 2>), grid, dim3(64), 0, stream, a, shift);
+    else if (many && a.n <= 512)
+      hipLaunchKernelGGL((draw_short_kernel<T, 64, 8>), grid, dim3(64), 0, stream, a, shift);
+    else if (a.n <= 512)
       hipLaunchKernelGGL((draw_short_kernel<T, 256, 2>), grid, dim3(256), 0, stream, a, shift);
-    else if (a.n <= 2048)
+    else if (many && a.n <= 2048)
       hipLaunchKernelGGL((draw_short_kernel<T, 256, 8>), grid, dim3(256), 0, stream, a, shift);
+    else if (a.n <= 2048)
+      hipLaunchKernelGGL((draw_short_kernel<T, 512, 4>), grid, dim3(512), 0, stream, a, shift);
+    else if (many)
+      hipLaunchKernelGGL((draw_short_kernel<T, 512, 16>), grid, dim3(512), 0, stream, a, shift);
     else
       hipLaunchKernelGGL((draw_short_kernel<T, 1024, 8>), grid, dim3(1024), 0, stream, a, shift);
   } else if (!p.vpt) {

@@ -53,6 +53,17 @@ __device__ __forceinline__ double wave_last(double v)
   return __longlong_as_double((long long)wave_last((unsigned long long)__double_as_longlong(v)));
 }
 
+// Lane `from`'s value (the same for all lanes).
+__device__ __forceinline__ uint32_t wave_lane(uint32_t v, int from) { return (uint32_t)__builtin_amdgcn_readlane((int)v, from); }
+__device__ __forceinline__ unsigned long long wave_lane(unsigned long long v, int from)
+{
+  return (unsigned long long)wave_lane((uint32_t)(v >> 32), from) << 32 | wave_lane((uint32_t)v, from);
+}
+__device__ __forceinline__ double wave_lane(double v, int from)
+{
+  return __longlong_as_double((long long)wave_lane((unsigned long long)__double_as_longlong(v), from));
+}
+
 // Running sum over the lanes up to and with this one.
 template <typename V> __device__ __forceinline__ V wave_running(V v)
 {
