@@ -102,6 +102,13 @@ int check_shape(int64_t rows, int64_t cols)
   return MHLIK_OK;
 }
 
+int check_workspace(const void *space, size_t bytes, size_t need)
+{
+  if (need && (!space || !aligned16(space) || bytes < need))
+    return fail_no_ctx(MHLIK_EINVAL, "workspace: %zu bytes at a multiple of 16 are needed (%zu given)", need, bytes);
+  return MHLIK_OK;
+}
+
 int check_values(const char *what, const void *x, int32_t type, int64_t rows, int64_t rs, int64_t cs)
 {
   if (!type_size(type)) return fail_no_ctx(MHLIK_EINVAL, "%s: unknown element type %d", what, type);
@@ -113,6 +120,11 @@ int check_values(const char *what, const void *x, int32_t type, int64_t rows, in
 
 // Rows that the few-rows kernel quantizes by itself.
 bool few_rows(int64_t rows, int64_t cols) { return rows <= 64 && rows * q8_blocks(cols) * kQ8Block <= kQ8FewBytes; }
+
+size_t product_space(int64_t rows, int64_t cols)
+{
+  return few_rows(rows, cols) ? 0 : (size_t)rows * (size_t)(q8_blocks(cols) * kQ8Block + q8_scale_stride(cols));
+}
 
 // values.type != 0: the rows are those (few_rows says that they are few enough), not a.x
 template <typename T> int product_launch(const Q8Product &a, const Q8Values &values, hipStream_t stream)
@@ -220,13 +232,11 @@ template <typename T, int VEC, int VPT> void draw_long(const DrawArgs &a, const 
   hipLaunchKernelGGL((draw_finish_kernel<T, VPT>), dim3((unsigned)a.rows), dim3(1024), 0, stream, a, g, shift);
 }
 
-template <typename T> int draw_launch(const DrawArgs &a, void *workspace, size_t workspace_bytes, hipStream_t stream)
+template <typename T> int draw_launch(const DrawArgs &a, void *workspace, hipStream_t stream)
 {
   int shift = 63; // weights in whole numbers: n of them stay below 2^63
   while (((int64_t)1 << (63 - shift)) < a.n) shift--;
   const DrawPlan p = draw_plan(a.rows, a.n, workspace);
-  if (p.bytes && (!aligned16(workspace) || !workspace || workspace_bytes < p.bytes))
-    return fail_no_ctx(MHLIK_EINVAL, "workspace: %zu bytes at a multiple of 16 are needed (%zu given)", p.bytes, workspace_bytes);
   if (p.short_rows) {
     // Many rows: few waves a row, since a wave's own cost (scans, the border) adds up (top-k, top-p and min-p, 4096 rows:
     // of 2000, 4 waves 39 us, 8 waves 47; of 400, 1 wave 14 us, 4 waves 20).  Few rows: as many waves as there is work
@@ -291,7 +301,7 @@ int mhlik_q8_product_workspace(int64_t rows, int64_t cols, size_t *bytes)
 {
   if (!bytes) return fail_no_ctx(MHLIK_EINVAL, "bytes must not be NULL");
   if (int rc = check_shape(rows, cols)) return rc;
-  *bytes = few_rows(rows, cols) ? 0 : (size_t)rows * (size_t)(q8_blocks(cols) * kQ8Block + q8_scale_stride(cols));
+  *bytes = product_space(rows, cols);
   return MHLIK_OK;
 }
 
@@ -313,6 +323,9 @@ int mhlik_q8_product(const mhlik_q8_operands *p, int32_t device, void *stream)
   if (!p->out || (uintptr_t)p->out % type_size(p->out_type)) return fail_no_ctx(MHLIK_EINVAL, "out is NULL or not aligned to its type");
   if (p->out_stride < p->draws)
     return fail_no_ctx(MHLIK_EINVAL, "out_stride=%lld is less than draws=%lld", (long long)p->out_stride, (long long)p->draws);
+  if (!ready) {
+    if (int rc = check_workspace(p->workspace, p->workspace_bytes, product_space(p->rows, p->cols))) return rc;
+  }
   OnDevice on(device);
   PCHK(on.err);
   Q8Product a;
@@ -334,9 +347,6 @@ int mhlik_q8_product(const mhlik_q8_operands *p, int32_t device, void *stream)
     values = Q8Values{p->x, p->x_row_stride, p->x_col_stride, p->x_type};
     a.x = a.xs = nullptr;
   } else {
-    const size_t need = (size_t)p->rows * (size_t)(a.kp + a.sstride);
-    if (!p->workspace || !aligned16(p->workspace) || p->workspace_bytes < need)
-      return fail_no_ctx(MHLIK_EINVAL, "workspace: %zu bytes at a multiple of 16 are needed (%zu given)", need, p->workspace_bytes);
     uint8_t *data = (uint8_t *)p->workspace, *scale = data + p->rows * a.kp;
     if (int rc = quantize(p->x, p->x_type, p->rows, p->cols, p->x_row_stride, p->x_col_stride, data, scale, (hipStream_t)stream)) return rc;
     a.x = data;
@@ -371,6 +381,7 @@ int mhlik_draw(const mhlik_draw_rows *p, int32_t device, void *stream)
   if (!p->top_p && p->top_p_all != p->top_p_all) return fail_no_ctx(MHLIK_EINVAL, "top_p is not a number");
   if (!p->min_p && p->min_p_all != p->min_p_all) return fail_no_ctx(MHLIK_EINVAL, "min_p is not a number");
   if (p->rows == 0) return MHLIK_OK;
+  if (int rc = check_workspace(p->workspace, p->workspace_bytes, draw_plan(p->rows, p->n, nullptr).bytes)) return rc;
   OnDevice on(device);
   PCHK(on.err);
   DrawArgs a;
@@ -391,9 +402,9 @@ int mhlik_draw(const mhlik_draw_rows *p, int32_t device, void *stream)
   a.index = p->index;
   a.logp = p->logp;
   switch (p->z_type) {
-  case MHLIK_T_F32: return draw_launch<float>(a, p->workspace, p->workspace_bytes, (hipStream_t)stream);
-  case MHLIK_T_BF16: return draw_launch<__bf16>(a, p->workspace, p->workspace_bytes, (hipStream_t)stream);
-  default: return draw_launch<_Float16>(a, p->workspace, p->workspace_bytes, (hipStream_t)stream);
+  case MHLIK_T_F32: return draw_launch<float>(a, p->workspace, (hipStream_t)stream);
+  case MHLIK_T_BF16: return draw_launch<__bf16>(a, p->workspace, (hipStream_t)stream);
+  default: return draw_launch<_Float16>(a, p->workspace, (hipStream_t)stream);
   }
 }
 }

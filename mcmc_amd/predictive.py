@@ -208,3 +208,56 @@ def draw(z, u, temperature=1.0, top_k=None, top_p=None, min_p=None):
     gpu = device.index
     _chk(L.load_mhlik().mhlik_draw(C.byref(p), gpu, _stream(gpu)))
     return index, logp
+
+
+class PosteriorPredictive:
+    """New observations under the draws that a sampler has kept: theta [draws, cols] (the `samples` of a sampler, or a
+    tensor), held in 8 bits on one GPU.
+
+    A predictor x.theta_s differs from the one in 32 bits by the rounding of x and theta_s to four significant bits, 2^-4
+    relative for each product at most and of either sign, so that averages over draws and columns lose most of it.  An
+    accept test would not: the samplers' likelihoods do not go through here."""
+
+    CHUNK = 1 << 26  # predictors held at a time
+
+    def __init__(self, theta, device=None):
+        theta = torch.as_tensor(theta)
+        if not theta.is_cuda or device is not None:
+            theta = theta.to("cuda" if device is None else device)
+        _need(theta.dim() == 2 and theta.shape[0] >= 1, "theta must have two dimensions and at least one draw")
+        self.theta = quantize(theta.detach())
+
+    def predictor(self, x, dtype=torch.float32):
+        """x_i.theta_s for every row of x [rows, cols] and every draw."""
+        return product(x, self.theta, dtype)
+
+    def _chunks(self, rows):
+        step = max(1, self.CHUNK // self.theta.rows)
+        return ((i, min(rows, i + step)) for i in range(0, rows, step))
+
+    def probability(self, x):
+        """P(y = 1 | x_i), float32 [rows]: the mean of 1 / (1 + exp(-x_i.theta_s)) over the draws."""
+        _given("x", x, 2, _TYPES)
+        out = torch.empty(x.shape[0], dtype=torch.float32, device=x.device)
+        for i, j in self._chunks(x.shape[0]):
+            torch.mean(torch.sigmoid(self.predictor(x[i:j])), 1, out=out[i:j])
+        return out
+
+    def case_deletion(self, x, u, temperature=1.0, top_k=None, top_p=None, min_p=None):
+        """For every observation a draw from the posterior without it: (draw int64 [rows], log probability [rows]).
+
+        x holds the observations with their labels folded in, as the samplers' design matrix does (-y_i x_i): then
+        1 / p(y_i | x_i, theta_s) = 1 + exp(x_i.theta_s) are the weights that take observation i out of the posterior.
+        u [rows] are random numbers in [0, 1); the other arguments flatten or cut the weights, see `draw`."""
+        _given("x", x, 2, _TYPES)
+        rows = x.shape[0]
+        _same("u", _given("u", u, 1, _U), x.device)
+        _need(u.shape[0] == rows, "u has %d values for %d rows", u.shape[0], rows)
+        choices = {"temperature": temperature, "top_k": top_k, "top_p": top_p, "min_p": min_p}
+        index = torch.empty(rows, dtype=torch.int64, device=x.device)
+        logp = torch.empty(rows, dtype=torch.float32, device=x.device)
+        zero = torch.zeros((), device=x.device)
+        for i, j in self._chunks(rows):
+            part = {k: v[i:j] if isinstance(v, torch.Tensor) else v for k, v in choices.items()}
+            index[i:j], logp[i:j] = draw(torch.logaddexp(self.predictor(x[i:j]), zero), u[i:j], **part)
+        return index, logp
