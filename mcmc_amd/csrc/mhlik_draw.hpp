@@ -55,8 +55,8 @@ __device__ __forceinline__ float draw_finite(float z) { return fminf(z, 0x1.ffff
 // 2^((z - max) s), s = log2(e) / T: 1 at z = max, within 5e-16 relative where it matters ((z - max) s is rounded: another
 // 1e-16 times itself), 0 below 2^-1020 and for z = -inf.  Whole part by adding 1.5 * 2^52, whose low bits then hold it;
 // the rest goes through the degree-10 polynomial of mhlik_exp_fast with the powers of ln 2 multiplied in: 17 double
-// instructions, of which none is slower than an addition.
-__device__ __forceinline__ double draw_weight(float z, float max, double s)
+// instructions, of which none is slower than an addition.  EXACT_ZERO false, for sums only: 2^-1020 in place of 0.
+template <bool EXACT_ZERO = true> __device__ __forceinline__ double draw_weight(float z, float max, double s)
 {
   MHLIK_SP_COEF(c10, 0x1.e364ae3ebe671p-28);
   MHLIK_SP_COEF(c9, 0x1.b660a93518429p-24);
@@ -68,7 +68,7 @@ __device__ __forceinline__ double draw_weight(float z, float max, double s)
   MHLIK_SP_COEF(c3, 0x1.c6b08d704396dp-5);
   MHLIK_SP_COEF(c2, 0x1.ebfbdff82c46cp-3);
   MHLIK_SP_COEF(c1, 0x1.62e42fefa39efp-1);
-  const double y = fmax(((double)z - (double)max) * s, -1100.0); // NaN (-inf * 0) too
+  const double y = fmax(((double)z - (double)max) * s, EXACT_ZERO ? -1100.0 : -1020.0); // NaN (-inf * 0) too
   const double m = y + 0x1.8p52, f = y - (m - 0x1.8p52);
   double p = fma(c10, f, c9);
   p = fma(p, f, c8);
@@ -81,7 +81,7 @@ __device__ __forceinline__ double draw_weight(float z, float max, double s)
   p = fma(p, f, c1);
   p = fma(p, f, 1.0);
   const double w = __hiloint2double(__double2hiint(p) + (int)((uint32_t)__double2loint(m) << 20), __double2loint(p));
-  return y < -1020.0 ? 0.0 : w;
+  return EXACT_ZERO && y < -1020.0 ? 0.0 : w;
 }
 
 // The choices of one row.
@@ -759,7 +759,7 @@ __global__ __launch_bounds__(kBlock) void draw_top_kernel(DrawArgs a, LongSpace 
     first = (int)wave_min((uint32_t)first);
   } else if (draw_kind(c, false, max) == kRowPlain) {
 #pragma unroll
-    for (int i = 0; i < VPT; i++) mass += draw_weight(z[i], max, c.rate);
+    for (int i = 0; i < VPT; i++) mass += draw_weight<false>(z[i], max, c.rate);
     mass = wave_sum(mass);
   }
   const bool any = __any(nan);

@@ -154,15 +154,23 @@ template <typename T> int product_launch(const Q8Product &a, const Q8Values &val
     else
       hipLaunchKernelGGL((q8_skinny_kernel<T, 4, false>), grid, block, 0, stream, a, values, ks);
   } else if (a.blocks <= 2) {
-    const int64_t gn = (a.draws + 255) / 256;
-    int64_t walk = 512; // rows a workgroup walks down: fewer where the chip would not be full
-    while (walk > 32 && (a.rows + walk - 1) / walk * gn < 2048) walk /= 2;
-    const int64_t gm = (a.rows + walk - 1) / walk;
-    if (gm * gn > INT32_MAX) return fail_no_ctx(MHLIK_EINVAL, "too large a product (%lld x %lld)", (long long)a.rows, (long long)a.draws);
-    if (a.blocks == 1)
-      hipLaunchKernelGGL((q8_thin_kernel<T, kWide, 1>), dim3((unsigned)(gm * gn)), dim3(kBlock), 0, stream, a, (int)gn, (int)walk);
+    const int64_t high = kBlock / kWave * 16 * q8_thin_down(a.blocks, sizeof(T)), gm = (a.rows + high - 1) / high;
+    const int64_t chunks = (a.draws + kQ8ThinDraws - 1) / kQ8ThinDraws;
+    int64_t splits = 1; // of the draws: until the chip's 256 CUs have four workgroups each, or those have one chunk
+    while (splits < chunks && gm * splits < 1024) splits++;
+    const int64_t each = (chunks + splits - 1) / splits;
+    splits = (chunks + each - 1) / each;
+    if (gm * splits > INT32_MAX) return fail_no_ctx(MHLIK_EINVAL, "too large a product (%lld x %lld)", (long long)a.rows, (long long)a.draws);
+    const dim3 grid((unsigned)(gm * splits));
+    const bool shifted = !aligned16(a.out) || a.os * (int64_t)sizeof(T) % 16 != 0; // rows that do not begin at 16 bytes
+    if (a.blocks == 1 && !shifted)
+      hipLaunchKernelGGL((q8_thin_kernel<T, kWide, 1, false>), grid, dim3(kBlock), 0, stream, a, (int)splits, (int)each);
+    else if (a.blocks == 1)
+      hipLaunchKernelGGL((q8_thin_kernel<T, kWide, 1, true>), grid, dim3(kBlock), 0, stream, a, (int)splits, (int)each);
+    else if (!shifted)
+      hipLaunchKernelGGL((q8_thin_kernel<T, kWide, 2, false>), grid, dim3(kBlock), 0, stream, a, (int)splits, (int)each);
     else
-      hipLaunchKernelGGL((q8_thin_kernel<T, kWide, 2>), dim3((unsigned)(gm * gn)), dim3(kBlock), 0, stream, a, (int)gn, (int)walk);
+      hipLaunchKernelGGL((q8_thin_kernel<T, kWide, 2, true>), grid, dim3(kBlock), 0, stream, a, (int)splits, (int)each);
   } else {
     // Tiles of 256 do a quarter of the fetching per product that tiles of 64 would, and half of what tiles of 128 do; from
     // where they fill three quarters of the chip's 256 CUs they are the faster ones.

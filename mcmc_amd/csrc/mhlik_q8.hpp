@@ -207,7 +207,7 @@ __global__ __launch_bounds__(kBlock) void q8_columns_kernel(const T *__restrict_
 //                        them: 1.6e-5 of the result's norm (measured, the same at 128 and 8192 columns), a
 //                        hundredth of what rounding C to bfloat16 costs and a tenth of float16's.
 // All 128 columns of a step share their scales, so which column goes to which place of the instruction is free as long
-// as both operands agree: a lane's 32 bytes are consecutive.
+// as both operands agree.
 
 __device__ __forceinline__ float q8_scale_value(uint32_t code) { return __uint_as_float(code << 23); } // 2^(code - 127)
 
@@ -219,6 +219,13 @@ __device__ __forceinline__ q8_b8 q8_widen(q8_i8 v, int s, float scale)
   const q8_b2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)v[2 * s + 1], scale, false);
   const q8_b2 d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)v[2 * s + 1], scale, true);
   return q8_b8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+// A lane's 32 bytes of a block: pieces g and 4 + g, 16 bytes each (four lanes read 64 consecutive bytes at a time).
+__device__ __forceinline__ q8_i8 q8_pieces(const uint8_t *block, int g)
+{
+  const q8_i4 lo = *(const q8_i4 *)(block + g * 16), hi = *(const q8_i4 *)(block + 64 + g * 16);
+  return q8_i8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
 }
 
 template <typename T> __device__ __forceinline__ T q8_round(float v) { return (T)v; }
@@ -251,8 +258,8 @@ struct Q8Product {
 };
 
 // Few rows (up to 16 a fragment, RF fragments): what bounds it is reading the draws once.  A wave takes 16 draws and every
-// ks-th block of 128 columns; its lanes load 32 consecutive bytes of a draw straight into the instruction's operand, 4
-// lanes a block, four blocks ahead of the four being multiplied.  The ks waves of a 16-draw group add up through LDS in
+// ks-th block of 128 columns; its lanes load a draw's bytes straight into the instruction's operand, 4 lanes a block, four
+// blocks ahead of the four being multiplied.  The ks waves of a 16-draw group add up through LDS in
 // wave order.  The draws are the instruction's rows, so that a lane ends with four consecutive values of one row of C.
 // FROM_VALUES: the rows come as values; each workgroup quantizes all of them into LDS (they are few: up to 16 KB) while
 // its first draws are on their way, which saves a kernel and its start.
@@ -268,15 +275,16 @@ __global__ __launch_bounds__(512) void q8_skinny_kernel(Q8Product a, Q8Values va
   const int kw = wave % ks, nw = blockDim.x / kWave;
   const int64_t j0 = ((int64_t)blockIdx.x * (nw / ks) + wave / ks) * 16;
   const int64_t jr = j0 + r < a.draws ? j0 + r : a.draws - 1; // past the end: the last draw again, not stored
-  const uint8_t *w = a.w + jr * a.kp + g * 32, *ws = a.ws + jr * a.sstride;
+  const uint8_t *w = a.w + jr * a.kp, *ws = a.ws + jr * a.sstride;
   constexpr int kAhead = 4;
   q8_i8 wn[kAhead];
   uint32_t sn[kAhead];
   auto fetch = [&](int b0) {
 #pragma unroll
     for (int q = 0; q < kAhead; q++) {
-      const int b = b0 + q * ks < a.blocks ? b0 + q * ks : a.blocks - 1;
-      wn[q] = *(const q8_i8 *)(w + (int64_t)b * kQ8Block);
+      const int b = b0 + q * ks;
+      if (b >= a.blocks) break;
+      wn[q] = q8_pieces(w + (int64_t)b * kQ8Block, g);
       sn[q] = ws[b];
     }
   };
@@ -299,7 +307,7 @@ __global__ __launch_bounds__(512) void q8_skinny_kernel(Q8Product a, Q8Values va
 #pragma unroll
   for (int f = 0; f < RF; f++) {
     const int64_t ir = f * 16 + r < a.rows ? f * 16 + r : a.rows - 1;
-    x[f] = (FROM_VALUES ? bytes : a.x) + ir * a.kp + g * 32;
+    x[f] = (FROM_VALUES ? bytes : a.x) + ir * a.kp;
     xs[f] = FROM_VALUES ? codes + ir * a.blocks : a.xs + ir * a.sstride;
   }
   q8_f4 acc[RF];
@@ -310,7 +318,7 @@ __global__ __launch_bounds__(512) void q8_skinny_kernel(Q8Product a, Q8Values va
     uint32_t sv[kAhead];
 #pragma unroll
     for (int q = 0; q < kAhead; q++) {
-      wv[q] = wn[q];
+      wv[q] = wn[q]; // those past the last block: never used
       sv[q] = sn[q];
     }
     if (b0 + kAhead * ks < a.blocks) fetch(b0 + kAhead * ks);
@@ -322,7 +330,7 @@ __global__ __launch_bounds__(512) void q8_skinny_kernel(Q8Product a, Q8Values va
       float xsv[RF];
 #pragma unroll
       for (int f = 0; f < RF; f++) {
-        xv[f] = *(const q8_i8 *)(x[f] + b * kQ8Block);
+        xv[f] = q8_pieces(x[f] + (int64_t)b * kQ8Block, g);
         xsv[f] = q8_scale_value(xs[f][b]);
       }
 #pragma unroll
@@ -354,66 +362,185 @@ __global__ __launch_bounds__(512) void q8_skinny_kernel(Q8Product a, Q8Values va
   }
 }
 
-// Narrow matrices (one or two blocks of columns: the samplers' own widths), many rows: C's bytes are what there is to
-// do.  A wave keeps 64 draws in registers and walks down the rows, 16 at a time, straight from memory into the
-// instruction's operand, the next 16 on their way; the four waves of a workgroup take neighbouring draws of the same rows.
-// Lane (r, g) holds bytes 16 g and 64 + 16 g of a block, so that four lanes read 64 consecutive bytes.  Fragment f of
-// the draws has draw 32 (f / 2) + 8 (i / 4) + 4 (f % 2) + i % 4 as its row i: a lane ends with two runs of eight values
-// of a row of C, four lanes with 64 consecutive bytes of a 16-bit type.
-template <typename T, bool WIDE, int BLOCKS>
-__global__ __launch_bounds__(kBlock) void q8_thin_kernel(Q8Product a, int groups_n, int walk)
+// Rows of C seldom start at a line of 128 bytes, and stores that end inside lines cost: 200000 rows of 1024 bfloat16 take
+// 96 us, rows of 1000 (16 bytes off a line more or less) took 164, of 1025 (2 bytes) 249.  So a lane's pieces of 16 bytes
+// are put together anew: brought to 16-byte words of memory (a funnel shift of a piece and the one before it, which the
+// lane 16 below has), and a word that belongs to the next line is held back for a step: each pair of stores then writes
+// one whole line of each row.  A step is 128 bytes of a row, eight pieces, two to each of the row's four lanes: g and
+// 4 + g of a 16-bit type, 2 g and 2 g + 1 of float (as the fragments leave them).
+typedef uint32_t q8_u4 __attribute__((ext_vector_type(4)));
+
+// Sixteen bytes of C: the four values of a, or the eight of a and b.
+template <typename T> __device__ __forceinline__ q8_u4 q8_word(q8_f4 a, q8_f4 b)
 {
-#if defined(__HIP_DEVICE_COMPILE__)
-  const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave, r = lane & 15, g = lane >> 4;
-  const int64_t j0 = (int64_t)(blockIdx.x % groups_n) * 256 + wave * 64;
-  const int64_t from = (int64_t)(blockIdx.x / groups_n) * walk;
-  const int64_t to = from + walk < a.rows ? from + walk : a.rows;
-  if (j0 >= a.draws) return;
-  auto fragment = [&](const uint8_t *p) {
-    const q8_i4 lo = *(const q8_i4 *)(p + g * 16), hi = *(const q8_i4 *)(p + 64 + g * 16);
-    return q8_i8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-  };
-  q8_i8 wv[BLOCKS][4];
-  uint32_t ws[BLOCKS][4];
-#pragma unroll
-  for (int f = 0; f < 4; f++) {
-    int64_t j = j0 + (f >> 1) * 32 + (r >> 2) * 8 + (f & 1) * 4 + (r & 3);
-    j = j < a.draws ? j : a.draws - 1;
-#pragma unroll
-    for (int b = 0; b < BLOCKS; b++) {
-      wv[b][f] = fragment(a.w + j * a.kp + b * kQ8Block);
-      ws[b][f] = a.ws[j * a.sstride + b];
-    }
+  if constexpr (sizeof(T) == 4) {
+    return __builtin_bit_cast(q8_u4, a);
+  } else {
+    typedef T Eight __attribute__((ext_vector_type(8)));
+    return __builtin_bit_cast(q8_u4, Eight{q8_round<T>(a[0]), q8_round<T>(a[1]), q8_round<T>(a[2]), q8_round<T>(a[3]), q8_round<T>(b[0]),
+                                           q8_round<T>(b[1]), q8_round<T>(b[2]), q8_round<T>(b[3])});
   }
-  constexpr int kDown = BLOCKS == 1 ? 4 : 2; // fragments of rows under way
-  q8_i8 xn[kDown][BLOCKS];
-  uint32_t sn[kDown][BLOCKS];
-  auto fetch = [&](int64_t i0) {
+}
+
+template <typename T> struct Q8RowWriter {
+  static constexpr int kWord = 16 / sizeof(T); // values
+  typedef q8_u4 Word;
+  T *word0;   // the 16-byte word in which the row begins
+  int shift;  // bytes of that word before the row
+  int len;    // values of the row
+  int place[2];
+  bool hold[2];
+  Word held[2], last; // words held back; the piece before this step's first (shifted rows)
+
+  __device__ __forceinline__ Q8RowWriter() {}
+  __device__ __forceinline__ void begin(T *row, int n, int g)
+  {
+    shift = (int)((uintptr_t)row & 15);
+    word0 = (T *)((uintptr_t)row & ~(uintptr_t)15);
+    len = n;
+    const int first = (int)((uintptr_t)row >> 4 & 7);
+    place[0] = sizeof(T) == 2 ? g : 2 * g;
+    place[1] = sizeof(T) == 2 ? 4 + g : 2 * g + 1;
 #pragma unroll
-    for (int d = 0; d < kDown; d++) {
-      const int64_t i = i0 + d * 16 + r < to ? i0 + d * 16 + r : to - 1;
+    for (int a = 0; a < 2; a++) {
+      hold[a] = first + place[a] >= 8;
+      held[a] = Word{0, 0, 0, 0};
+    }
+    last = Word{0, 0, 0, 0};
+  }
+  // bytes 16 - shift .. 31 - shift of before:piece
+  __device__ __forceinline__ Word shifted(Word before, Word piece) const
+  {
+    const int off = 16 - shift, dw = off >> 2;
+    const bool two = dw & 2, one = dw & 1; // dw is 4 only without a shift
+    const uint32_t w0 = two ? before[2] : before[0], w1 = two ? before[3] : before[1], w2 = two ? piece[0] : before[2],
+                   w3 = two ? piece[1] : before[3], w4 = two ? piece[2] : piece[0], w5 = two ? piece[3] : piece[1];
+    const uint32_t x0 = one ? w1 : w0, x1 = one ? w2 : w1, x2 = one ? w3 : w2, x3 = one ? w4 : w3, x4 = one ? w5 : w4;
+    const Word o = {__builtin_amdgcn_alignbyte(x1, x0, off & 3), __builtin_amdgcn_alignbyte(x2, x1, off & 3),
+                    __builtin_amdgcn_alignbyte(x3, x2, off & 3), __builtin_amdgcn_alignbyte(x4, x3, off & 3)};
+    return shift ? o : piece;
+  }
+  // Step t's two pieces.  SHIFTED: some row does not begin at 16 bytes.  WHOLE: every word of this step lies within the row.
+  template <bool WHOLE, bool SHIFTED> __device__ __forceinline__ void step(int t, Word piece0, Word piece1, int g)
+  {
+    Word word[2] = {piece0, piece1};
+    if (SHIFTED) {
+      const int from = (((int)threadIdx.x + 48) & 63) * 4;
+      Word up0, up1;
 #pragma unroll
-      for (int b = 0; b < BLOCKS; b++) {
-        xn[d][b] = fragment(a.x + i * a.kp + b * kQ8Block);
-        sn[d][b] = a.xs[i * a.sstride + b];
+      for (int i = 0; i < 4; i++) {
+        up0[i] = sizeof(T) == 2 ? (uint32_t)__builtin_amdgcn_ds_bpermute(from, (int)piece0[i]) : 0u;
+        up1[i] = (uint32_t)__builtin_amdgcn_ds_bpermute(from, (int)piece1[i]);
+      }
+      const Word before0 = g == 0 ? last : sizeof(T) == 2 ? up0 : up1;
+      const Word before1 = sizeof(T) == 2 ? (g == 0 ? up0 : up1) : piece0;
+      word[0] = shifted(before0, piece0);
+      word[1] = shifted(before1, piece1);
+      last = up1;
+    }
+#pragma unroll
+    for (int a = 0; a < 2; a++) {
+      const Word o = hold[a] ? held[a] : word[a];
+      const int w = (hold[a] ? t - 1 : t) * 8 + place[a];
+      held[a] = word[a];
+      if (WHOLE) {
+        *(Word *)(word0 + w * kWord) = o;
+      } else {
+        const int e = w * kWord - (SHIFTED ? shift / (int)sizeof(T) : 0);
+        if (e >= 0 && e + kWord <= len) {
+          *(Word *)(word0 + w * kWord) = o;
+        } else if (e > -kWord && e < len) {
+          typedef T Values __attribute__((ext_vector_type(kWord)));
+          const Values v = __builtin_bit_cast(Values, o);
+#pragma unroll
+          for (int i = 0; i < kWord; i++)
+            if (e + i >= 0 && e + i < len) word0[w * kWord + i] = v[i];
+        }
       }
     }
-  };
-  // WHOLE: the wave's 64 draws are all there.  Rows past the end are the last one again and are stored as such, so that no
-  // branch lies between a fetch and its use: the wait for it would be one for the stores as well (one counter for both).
-  auto walk_down = [&](auto whole) {
-    fetch(from);
-    for (int64_t i0 = from; i0 < to; i0 += kDown * 16) {
-      q8_i8 xv[kDown][BLOCKS];
-      uint32_t xs[kDown][BLOCKS];
+  }
+};
+
+// Narrow matrices (one or two blocks of columns: the samplers' own widths), many rows: C's bytes are what there is to
+// do.  A wave keeps 64 rows (two blocks: 32) in registers and goes along the draws; a workgroup's four waves have rows
+// of their own and share the draws, 128 at a time, in LDS, the next 128 on their way: few loads, since loads queue behind
+// the stores (every wave fetching its own draws into registers: 154 us for 200000 x 1024 bfloat16, of which 77 for the
+// stores alone, 45 the loads, 35 the products, one after the other; this way 97).
+// Lane (r, g) holds pieces g and 4 + g, 16 bytes each, of a row's block.  Fragment f of 64 draws has draw 32 (f / 2) +
+// 8 (i / 4) + 4 (f % 2) + i % 4 as its row i: a lane ends with two runs of eight values of a row of C, four lanes with 64
+// consecutive bytes of a 16-bit type.  In LDS the pieces of draw d are ordered by a key of d, so that the lanes that a
+// ds_read_b128 serves together touch different banks.
+constexpr int kQ8ThinDraws = 128;
+
+// Fragments of 16 rows a wave has: as many as leave registers for two waves a SIMD.
+__host__ __device__ constexpr int q8_thin_down(int blocks, int size) { return blocks == 1 ? (size == 2 ? 4 : 2) : size == 2 ? 2 : 1; }
+
+template <typename T, bool WIDE, int BLOCKS, bool SHIFTED>
+__global__ __launch_bounds__(kBlock, 2) void q8_thin_kernel(Q8Product a, int splits, int chunks)
+{
+#if defined(__HIP_DEVICE_COMPILE__)
+  constexpr int kDown = q8_thin_down(BLOCKS, (int)sizeof(T)), kN = kQ8ThinDraws; // draws at a time
+  constexpr int kSide = kN * kQ8Block;
+  constexpr int kStores = kN / 64 * kDown * 2 * (int)sizeof(T) / 2; // a wave's, for one chunk of draws
+  __shared__ __align__(1024) uint8_t lds[2][BLOCKS * kSide];
+  __shared__ __align__(1024) uint32_t lds_scale[2][kN];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x % kWave, r = lane & 15, g = lane >> 4;
+  const int64_t i0 = ((int64_t)(blockIdx.x / splits) * (kBlock / kWave) + wave) * kDown * 16;
+  const int64_t from = (int64_t)(blockIdx.x % splits) * chunks * kN;
+  const int64_t to = from + (int64_t)chunks * kN < a.draws ? from + (int64_t)chunks * kN : a.draws;
+
+  q8_i8 xv[kDown][BLOCKS];
+  uint32_t xs[kDown][BLOCKS];
+  Q8RowWriter<T> out[kDown];
 #pragma unroll
-      for (int d = 0; d < kDown; d++)
+  for (int d = 0; d < kDown; d++) { // rows past the end: the last one again, and stored as such
+    const int64_t i = i0 + d * 16 + r < a.rows ? i0 + d * 16 + r : a.rows - 1;
+    out[d].begin((T *)a.out + i * a.os + from, (int)(to - from), g);
+#pragma unroll
+    for (int b = 0; b < BLOCKS; b++) {
+      xv[d][b] = q8_pieces(a.x + i * a.kp + b * kQ8Block, g);
+      xs[d][b] = a.xs[i * a.sstride + b];
+    }
+  }
+
+  auto key = [](int d) { return (d & 3) | ((d >> 3) & 1) << 2; };
+  auto fetch = [&](int buf, int64_t j0) { // a wave brings a quarter of the draws, eight draws of a block at once
+    const int last = (int)(a.draws - j0 < kN ? a.draws - j0 : kN) - 1, kp = (int)a.kp;
+    const __amdgpu_buffer_rsrc_t wr = __builtin_amdgcn_make_buffer_rsrc((void *)(a.w + j0 * a.kp), 0, (last + 1) * kp, 0x00020000);
+#pragma unroll
+    for (int q = 0; q < kN / 32; q++) {
+      const int d = (wave * (kN / 32) + q) * 8 + (lane >> 3);
+      const int at = (d < last ? d : last) * kp + ((lane & 7) ^ key(d)) * 16;
+#pragma unroll
+      for (int b = 0; b < BLOCKS; b++)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(wr, (__attribute__((address_space(3))) void *)(lds[buf] + b * kSide + (wave * (kN / 32) + q) * 1024), 16, at,
+                                                 b * kQ8Block, 0, 0);
+    }
+    if (wave < kN / kWave) { // the word that holds the scales of a draw's first four blocks
+      const __amdgpu_buffer_rsrc_t sr = __builtin_amdgcn_make_buffer_rsrc((void *)(a.ws + j0 * a.sstride), 0, (last + 1) * a.sstride, 0x00020000);
+      const int d = wave * kWave + lane;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(sr, (__attribute__((address_space(3))) void *)(lds_scale[buf] + wave * kWave), 4, (d < last ? d : last) * a.sstride, 0, 0, 0);
+    }
+  };
+
+  const int wl = (r >> 2) * 8 + (r & 3); // this lane's draw of fragment 0; the others have the same key
+  typedef typename Q8RowWriter<T>::Word Word;
+  auto chunk = [&](int buf, int t0, auto whole) {
+#pragma unroll 1
+    for (int h = 0; h < kN; h += 64) {
+      q8_i8 wv[BLOCKS][4];
+      uint32_t ws[4];
+#pragma unroll
+      for (int f = 0; f < 4; f++) {
+        const int d = h + (f >> 1) * 32 + (f & 1) * 4 + wl;
+        ws[f] = lds_scale[buf][d];
 #pragma unroll
         for (int b = 0; b < BLOCKS; b++) {
-          xv[d][b] = xn[d][b];
-          xs[d][b] = sn[d][b];
+          const uint8_t *p = lds[buf] + b * kSide + d * kQ8Block;
+          const q8_i4 lo = *(const q8_i4 *)(p + (g ^ key(wl)) * 16), hi = *(const q8_i4 *)(p + ((4 + g) ^ key(wl)) * 16);
+          wv[b][f] = q8_i8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
         }
-      fetch(i0 + kDown * 16);
+      }
 #pragma unroll
       for (int d = 0; d < kDown; d++) {
         q8_f4 acc[4];
@@ -427,28 +554,50 @@ __global__ __launch_bounds__(kBlock) void q8_thin_kernel(Q8Product a, int groups
               const q8_b8 xb = q8_widen(xv[d][b], s, q8_scale_value(xs[d][b]));
 #pragma unroll
               for (int f = 0; f < 4; f++)
-                acc[f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(q8_widen(wv[b][f], s, q8_scale_value(ws[b][f])), xb, acc[f], 0, 0, 0);
+                acc[f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(q8_widen(wv[b][f], s, q8_scale_value(ws[f] >> (8 * b) & 255u)), xb, acc[f], 0, 0, 0);
             }
           } else {
 #pragma unroll
             for (int f = 0; f < 4; f++)
-              acc[f] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wv[b][f], xv[d][b], acc[f], 0, 0, 0, (int)ws[b][f], 0, (int)xs[d][b]);
+              acc[f] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wv[b][f], xv[d][b], acc[f], 0, 0, 0, (int)(ws[f] >> (8 * b)), 0, (int)xs[d][b]);
           }
         }
-        const int64_t i = i0 + d * 16 + r < to ? i0 + d * 16 + r : to - 1;
 #pragma unroll
-        for (int f = 0; f < 4; f += 2) {
-          const int64_t j = j0 + (f >> 1) * 32 + g * 8;
-          const float v[8] = {acc[f][0], acc[f][1], acc[f][2], acc[f][3], acc[f + 1][0], acc[f + 1][1], acc[f + 1][2], acc[f + 1][3]};
-          if (whole.value || j < a.draws) q8_store<T, 8>((T *)a.out + i * a.os + j, v, whole.value ? 8 : a.draws - j);
+        for (int q = 0; q < (int)sizeof(T) / 2; q++) { // 64 values of a row are 16 sizeof(T) words over its four lanes
+          const Word p0 = q8_word<T>(acc[sizeof(T) == 2 ? 0 : 2 * q], acc[1]), p1 = q8_word<T>(acc[sizeof(T) == 2 ? 2 : 2 * q + 1], acc[3]);
+          const int t = t0 + h * (int)sizeof(T) / 128 + q;
+          if (whole.value || (t > 0 && (t + 1) * 8 * Q8RowWriter<T>::kWord <= (int)(to - from))) // the same for all lanes
+            out[d].template step<true, SHIFTED>(t, p0, p1, g);
+          else
+            out[d].template step<false, SHIFTED>(t, p0, p1, g);
         }
       }
     }
   };
-  if (j0 + 64 <= a.draws)
-    walk_down(std::true_type{});
-  else
-    walk_down(std::false_type{});
+
+  constexpr int kSteps = kN * (int)sizeof(T) / 128; // of the row writers, for one chunk
+  fetch(0, from);
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  int buf = 0, t = 0;
+  for (int64_t j0 = from; j0 < to; j0 += kN, buf ^= 1, t += kSteps) {
+    const bool more = j0 + kN < to;
+    if (more) fetch(buf ^ 1, j0 + kN);
+    if (t > 0 && j0 + kN <= to)
+      chunk(buf, t, std::true_type{});
+    else
+      chunk(buf, t, std::false_type{});
+    if (more) {
+      // the fetch is older than this chunk's stores, which need not be waited for (the first chunk's number varies)
+      if (t > 0)
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(kStores) : "memory");
+      else
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+      __builtin_amdgcn_s_barrier();
+    }
+  }
+#pragma unroll
+  for (int d = 0; d < kDown; d++) out[d].template step<false, SHIFTED>(t, Word{0, 0, 0, 0}, Word{0, 0, 0, 0}, g); // what is held
 #endif
 }
 
