@@ -626,8 +626,9 @@ __device__ __forceinline__ void q8_tile_of(int id, int tiles, int tiles_n, int *
   const int t = die * full + (die < rest ? die : rest) + id / 8;
   const int run = 4 * tiles_n, first = t / run * 4, tiles_m = tiles / tiles_n;
   const int high = tiles_m - first < 4 ? tiles_m - first : 4, in = t % run;
-  *tm = first + in % high;
-  *tn = in / high;
+  // in scalar registers: the buffer descriptors are built from them (from vector registers each load becomes a loop)
+  *tm = __builtin_amdgcn_readfirstlane(first + in % high);
+  *tn = __builtin_amdgcn_readfirstlane(in / high);
 }
 
 template <typename T, bool WIDE, int B>
