@@ -396,7 +396,7 @@ template <typename T> struct Q8RowWriter {
   __device__ __forceinline__ void begin(T *row, int n, int g)
   {
     shift = (int)((uintptr_t)row & 15);
-    word0 = (T *)((uintptr_t)row & ~(uintptr_t)15);
+    word0 = row - shift / (int)sizeof(T); // (from the row, so that the compiler still knows it for global memory)
     len = n;
     const int first = (int)((uintptr_t)row >> 4 & 7);
     place[0] = sizeof(T) == 2 ? g : 2 * g;
