@@ -453,14 +453,15 @@ enum { MHLIK_T_Q8 = 0, MHLIK_T_F64 = 1, MHLIK_T_F32 = 2, MHLIK_T_BF16 = 3, MHLIK
  * data has 128 ceil(cols/128) bytes a row (columns past the last: 0), starts at a multiple of 16 bytes; scale has
  * 4 ceil(cols/512) bytes a row (spare ones: 127).  Values that are not finite, or exceed 448 2^119, become NaN.
  * x[i * row_stride + c * col_stride], of any type but MHLIK_T_Q8; strides count elements and are not negative.
- * 0 <= rows <= 2^40, 1 <= cols <= 2^22. */
+ * 0 <= rows <= 2^40, 1 <= cols <= 2^22.  Rows made elsewhere: scale bytes 31 .. 246, as these k have. */
 int mhlik_q8_quantize(const void *x, int32_t type, int64_t rows, int64_t cols, int64_t row_stride, int64_t col_stride,
                       uint8_t *data, uint8_t *scale, int32_t device, void *stream);
 
 /* out[i * out_stride + s] = sum_c x[i][c] w[s][c] over the values that the 8-bit rows stand for.  x may be 8-bit rows
  * (x_type MHLIK_T_Q8: x and x_scale) or values, which are quantized first, into the workspace.  out is float (products
  * and sums as exact as float sums are), bfloat16 or half (products as the 8-bit matrix instructions add them: 1.6e-5 of
- * the result's norm before the rounding).  The padding of 8-bit rows must be zeros, and out must not overlap the inputs. */
+ * the result's norm before the rounding).  The padding of 8-bit rows must be zeros, and out must not overlap the inputs.
+ * 0 <= draws <= 2^29. */
 typedef struct mhlik_q8_operands {
   const void *x;          /* [rows] */
   const uint8_t *x_scale; /* MHLIK_T_Q8 only */

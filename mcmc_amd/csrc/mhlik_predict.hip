@@ -55,6 +55,12 @@ bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
 // 256 rows of a matrix are reached with 31-bit offsets
 constexpr int64_t kMaxCols = (int64_t)1 << 22;
 constexpr int64_t kMaxRows = (int64_t)1 << 40;
+constexpr int64_t kMaxDraws = (int64_t)1 << 29;
+// A launch has fewer than 2^32 threads; larger calls go in parts, one after the other on the stream.
+constexpr int64_t kPartRows = (int64_t)1 << 28;     // of a product or a quantization: 4 threads a row at most, or
+constexpr int64_t kPartBlocks = (int64_t)1 << 27;   // 16 a block
+constexpr int64_t kPartDrawRows = (int64_t)1 << 20; // of a draw: 1024 threads a row
+constexpr int64_t kPartWeights = (int64_t)1 << 27;  // of a draw's long rows, which bounds its workspace (1.1 GB)
 
 int check_rows8(const char *what, const void *data, const void *scale, int64_t rows)
 {
@@ -69,18 +75,20 @@ int quantize_launch(const T *x, int64_t rows, int64_t cols, int64_t rs, int64_t 
   const int64_t blocks = q8_blocks(cols), sstride = q8_scale_stride(cols);
   // Column by column if columns are contiguous and there are rows enough for a wave's loads to be (a wave of the row
   // kernel would touch 64 lines for 64 values); a single row is both: the row kernel spreads it over more lanes.
-  if (rs == 1 && cs != 1 && rows >= 16) {
-    const int64_t groups = (rows + kBlock - 1) / kBlock;
-    if (groups > INT32_MAX || blocks > 65535) return fail_no_ctx(MHLIK_EINVAL, "too many rows or columns (%lld x %lld)", (long long)rows, (long long)cols);
-    hipLaunchKernelGGL(q8_columns_kernel<T>, dim3((unsigned)groups, (unsigned)blocks), dim3(kBlock), 0, stream, x, rows, cols, cs,
-                       (uint32_t)blocks, (uint32_t)sstride, data, scale);
-  } else {
-    const int64_t units = rows * blocks, groups = (units * 16 + kBlock - 1) / kBlock;
-    if (groups > INT32_MAX) return fail_no_ctx(MHLIK_EINVAL, "too many blocks (%lld)", (long long)units);
-    hipLaunchKernelGGL(q8_rows_kernel<T>, dim3((unsigned)groups), dim3(kBlock), 0, stream, Q8Values{x, rs, cs, 0}, units, cols,
-                       (uint32_t)blocks, (uint32_t)sstride, data, scale);
+  const bool by_column = rs == 1 && cs != 1 && rows >= 16;
+  const int64_t part = by_column ? kPartRows : kPartBlocks / blocks; // at least 2^12: blocks <= 2^15
+  for (int64_t first = 0; first < rows; first += part) {
+    const int64_t n = std::min(part, rows - first);
+    const T *from = x + first * rs;
+    uint8_t *d = data + first * blocks * kQ8Block, *s = scale + first * sstride;
+    if (by_column)
+      hipLaunchKernelGGL(q8_columns_kernel<T>, dim3((unsigned)((n + kBlock - 1) / kBlock), (unsigned)blocks), dim3(kBlock), 0, stream, from,
+                         n, cols, cs, (uint32_t)blocks, (uint32_t)sstride, d, s);
+    else
+      hipLaunchKernelGGL(q8_rows_kernel<T>, dim3((unsigned)((n * blocks * 16 + kBlock - 1) / kBlock)), dim3(kBlock), 0, stream,
+                         Q8Values{from, rs, cs, 0}, n * blocks, cols, (uint32_t)blocks, (uint32_t)sstride, d, s);
+    PCHK(hipGetLastError());
   }
-  PCHK(hipGetLastError());
   return MHLIK_OK;
 }
 
@@ -127,7 +135,7 @@ size_t product_space(int64_t rows, int64_t cols)
 }
 
 // values.type != 0: the rows are those (few_rows says that they are few enough), not a.x
-template <typename T> int product_launch(const Q8Product &a, const Q8Values &values, hipStream_t stream)
+template <typename T> int product_part(const Q8Product &a, const Q8Values &values, hipStream_t stream)
 {
   constexpr bool kWide = sizeof(T) == 4;
   // Up to 64 rows a wave keeps all of them beside 16 draws, so that the draws are read once for all rows; more rows go
@@ -139,7 +147,6 @@ template <typename T> int product_launch(const Q8Product &a, const Q8Values &val
     while (ks < 8 && groups16 * ks < 4096 && a.blocks >= 4 * ks) ks *= 2;
     const int waves = ks < 4 ? 4 : ks;
     const int64_t groups = (groups16 + waves / ks - 1) / (waves / ks);
-    if (groups > INT32_MAX) return fail_no_ctx(MHLIK_EINVAL, "too many draws (%lld)", (long long)a.draws);
     const dim3 grid((unsigned)groups), block(waves * kWave);
     if (values.type && rf == 1)
       hipLaunchKernelGGL((q8_skinny_kernel<T, 1, true>), grid, block, 0, stream, a, values, ks);
@@ -160,7 +167,6 @@ template <typename T> int product_launch(const Q8Product &a, const Q8Values &val
     while (splits < chunks && gm * splits < 1024) splits++;
     const int64_t each = (chunks + splits - 1) / splits;
     splits = (chunks + each - 1) / each;
-    if (gm * splits > INT32_MAX) return fail_no_ctx(MHLIK_EINVAL, "too large a product (%lld x %lld)", (long long)a.rows, (long long)a.draws);
     const dim3 grid((unsigned)(gm * splits));
     const bool shifted = !aligned16(a.out) || a.os * (int64_t)sizeof(T) % 16 != 0; // rows that do not begin at 16 bytes
     if (a.blocks == 1 && !shifted)
@@ -176,7 +182,8 @@ template <typename T> int product_launch(const Q8Product &a, const Q8Values &val
     // where they fill three quarters of the chip's 256 CUs they are the faster ones.
     const int64_t big = ((a.rows + 255) / 256) * ((a.draws + 255) / 256);
     const int64_t side = big >= 192 ? 256 : 128, tm = (a.rows + side - 1) / side, tn = (a.draws + side - 1) / side;
-    if (tm * tn > INT32_MAX) return fail_no_ctx(MHLIK_EINVAL, "too large a product (%lld x %lld)", (long long)a.rows, (long long)a.draws);
+    if (tm * tn >= (int64_t)1 << 24) // 10^12 results
+      return fail_no_ctx(MHLIK_EINVAL, "too large a product (%lld x %lld)", (long long)a.rows, (long long)a.draws);
     const dim3 grid((unsigned)(tm * tn));
     if (side == 256)
       hipLaunchKernelGGL((q8_tile_kernel<T, kWide, 256>), grid, dim3(kBlock), 0, stream, a, (int)tn, (int)(tm * tn));
@@ -187,12 +194,26 @@ template <typename T> int product_launch(const Q8Product &a, const Q8Values &val
   return MHLIK_OK;
 }
 
+template <typename T> int product_launch(Q8Product a, const Q8Values &values, hipStream_t stream)
+{
+  const int64_t rows = a.rows;
+  for (int64_t left = rows; left > 0; left -= kPartRows) {
+    a.rows = std::min(left, kPartRows);
+    if (int rc = product_part<T>(a, values, stream)) return rc;
+    a.x += a.rows * a.kp; // (more than one part has 8-bit rows)
+    a.xs += a.rows * a.sstride;
+    a.out = (T *)a.out + a.rows * a.os;
+  }
+  return MHLIK_OK;
+}
+
 // How a batch of rows is drawn from.
 struct DrawPlan {
   int vpt = 0;     // long rows: values a lane of a unit holds; 0: rows that fit a workgroup, or too long for units
   bool short_rows = false;
   LongSpace space;
   size_t bytes = 0;
+  int64_t part = 0; // rows at a time
 };
 
 constexpr int kShortMax = 8192;  // columns that fit a workgroup's registers (1024 threads, 8 each)
@@ -202,7 +223,9 @@ DrawPlan draw_plan(int64_t rows, int64_t n, void *workspace)
 {
   DrawPlan p;
   p.short_rows = n <= kShortMax;
+  p.part = kPartDrawRows;
   if (p.short_rows) return p;
+  if (n <= kLongVpt * kWave * kLongUnits) rows = p.part = std::min(rows, std::max<int64_t>(1, kPartWeights / n));
   p.vpt = rows * ((n + kLongVpt * kWave - 1) / (kLongVpt * kWave)) < 2048 && n <= (int64_t)8 * kWave * kLongUnits ? 8 : kLongVpt;
   const int64_t unit = p.vpt * kWave, units = (n + unit - 1) / unit;
   if (units > kLongUnits) {
@@ -240,11 +263,8 @@ template <typename T, int VEC, int VPT> void draw_long(const DrawArgs &a, const 
   hipLaunchKernelGGL((draw_finish_kernel<T, VPT>), dim3((unsigned)a.rows), dim3(1024), 0, stream, a, g, shift);
 }
 
-template <typename T> int draw_launch(const DrawArgs &a, void *workspace, hipStream_t stream)
+template <typename T> int draw_part(const DrawArgs &a, const DrawPlan &p, int shift, hipStream_t stream)
 {
-  int shift = 63; // weights in whole numbers: n of them stay below 2^63
-  while (((int64_t)1 << (63 - shift)) < a.n) shift--;
-  const DrawPlan p = draw_plan(a.rows, a.n, workspace);
   if (p.short_rows) {
     // Many rows: few waves a row, since a wave's own cost (scans, the border) adds up (top-k, top-p and min-p, 4096 rows:
     // of 2000, 4 waves 39 us, 8 waves 47; of 400, 1 wave 14 us, 4 waves 20).  Few rows: as many waves as there is work
@@ -268,8 +288,6 @@ template <typename T> int draw_launch(const DrawArgs &a, void *workspace, hipStr
   } else if (!p.vpt) {
     hipLaunchKernelGGL(draw_huge_kernel<T>, dim3((unsigned)a.rows), dim3(1024), 0, stream, a, shift);
   } else {
-    if (a.rows * p.space.groups > INT32_MAX)
-      return fail_no_ctx(MHLIK_EINVAL, "too many rows of this length (%lld x %lld)", (long long)a.rows, (long long)a.n);
     const bool histo = a.top_k || a.top_p || (a.top_k_all > 0 && a.top_k_all < a.n) || a.top_p_all < 1.0;
     const bool collect = histo || a.min_p || a.min_p_all > 0.0;
     constexpr int kVec = 16 / sizeof(T);
@@ -279,6 +297,25 @@ template <typename T> int draw_launch(const DrawArgs &a, void *workspace, hipStr
       draw_long<T, kVec, kLongVpt>(a, p.space, shift, histo, collect, stream);
   }
   PCHK(hipGetLastError());
+  return MHLIK_OK;
+}
+
+template <typename T> int draw_launch(DrawArgs a, const DrawPlan &p, hipStream_t stream)
+{
+  int shift = 63; // weights in whole numbers: n of them stay below 2^63
+  while (((int64_t)1 << (63 - shift)) < a.n) shift--;
+  for (int64_t left = a.rows; left > 0; left -= p.part) {
+    const int64_t rows = a.rows = std::min(left, p.part);
+    if (int rc = draw_part<T>(a, p, shift, stream)) return rc;
+    a.z = (const T *)a.z + rows * a.stride;
+    a.u = (const char *)a.u + rows * (a.u_is_double ? 8 : 4);
+    if (a.temperature) a.temperature += rows;
+    if (a.top_k) a.top_k += rows;
+    if (a.top_p) a.top_p += rows;
+    if (a.min_p) a.min_p += rows;
+    a.index += rows;
+    if (a.logp) a.logp += rows;
+  }
   return MHLIK_OK;
 }
 
@@ -317,7 +354,7 @@ int mhlik_q8_product(const mhlik_q8_operands *p, int32_t device, void *stream)
 {
   if (!p) return fail_no_ctx(MHLIK_EINVAL, "operands must not be NULL");
   if (int rc = check_shape(p->rows, p->cols)) return rc;
-  if (int rc = check_shape(p->draws, p->cols)) return rc;
+  if (p->draws < 0 || p->draws > kMaxDraws) return fail_no_ctx(MHLIK_EINVAL, "need 0 <= rows <= 2^40 and 0 <= draws <= 2^29 (draws=%lld)", (long long)p->draws);
   if (int rc = check_rows8("w", p->w_data, p->w_scale, p->draws)) return rc;
   const bool ready = p->x_type == MHLIK_T_Q8;
   if (ready) {
@@ -389,7 +426,8 @@ int mhlik_draw(const mhlik_draw_rows *p, int32_t device, void *stream)
   if (!p->top_p && p->top_p_all != p->top_p_all) return fail_no_ctx(MHLIK_EINVAL, "top_p is not a number");
   if (!p->min_p && p->min_p_all != p->min_p_all) return fail_no_ctx(MHLIK_EINVAL, "min_p is not a number");
   if (p->rows == 0) return MHLIK_OK;
-  if (int rc = check_workspace(p->workspace, p->workspace_bytes, draw_plan(p->rows, p->n, nullptr).bytes)) return rc;
+  const DrawPlan plan = draw_plan(p->rows, p->n, p->workspace);
+  if (int rc = check_workspace(p->workspace, p->workspace_bytes, plan.bytes)) return rc;
   OnDevice on(device);
   PCHK(on.err);
   DrawArgs a;
@@ -410,9 +448,9 @@ int mhlik_draw(const mhlik_draw_rows *p, int32_t device, void *stream)
   a.index = p->index;
   a.logp = p->logp;
   switch (p->z_type) {
-  case MHLIK_T_F32: return draw_launch<float>(a, p->workspace, (hipStream_t)stream);
-  case MHLIK_T_BF16: return draw_launch<__bf16>(a, p->workspace, (hipStream_t)stream);
-  default: return draw_launch<_Float16>(a, p->workspace, (hipStream_t)stream);
+  case MHLIK_T_F32: return draw_launch<float>(a, plan, (hipStream_t)stream);
+  case MHLIK_T_BF16: return draw_launch<__bf16>(a, plan, (hipStream_t)stream);
+  default: return draw_launch<_Float16>(a, plan, (hipStream_t)stream);
   }
 }
 }

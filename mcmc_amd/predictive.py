@@ -55,7 +55,8 @@ _stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index:
 
 class Block8:
     """Rows of `cols` values in 8 bits: `data` float8_e4m3fn [rows, 128 ceil(cols / 128)], columns past the last 0, and
-    `scale` uint8 [rows, 4 ceil(cols / 512)]: the 128 columns of block b stand for data * 2^(scale[:, b] - 127)."""
+    `scale` uint8 [rows, 4 ceil(cols / 512)]: the 128 columns of block b stand for data * 2^(scale[:, b] - 127), with
+    scales from 31 to 246."""
 
     __slots__ = ("data", "scale", "cols", "rows", "device")
 

@@ -345,6 +345,30 @@ def test_draw_ties(P, n):
             check_draw(P, z, u, **choice)
 
 
+@pytest.mark.parametrize("n", [100, 400, 1500, 3000])
+def test_draw_many_rows_of_ties(P, n):
+    """Fewer waves take a row when there are many; the border falls among hundreds of equal weights."""
+    g = torch.Generator(device="cuda").manual_seed(17 * n)
+    rows = 515
+    z = torch.randint(-2, 2, (rows, n), generator=g, device="cuda").float()
+    u = torch.rand(rows, generator=g, device="cuda", dtype=torch.float64)
+    check_draw(P, z, u, top_k=n // 3)
+    check_draw(P, z.bfloat16(), u, top_p=0.7)
+    check_draw(P, z, u, temperature=2.0, top_k=2 * n // 3, top_p=0.5, min_p=0.1)
+
+
+@pytest.mark.parametrize("rows,n", [(3, 100), (3, 3000), (3, 20000), (515, 100), (515, 400), (515, 1500), (515, 3000)])
+def test_draw_border_among_crowded_weights(P, rows, n):
+    """One weight far above the rest, which lie so close together that no histogram tells them apart."""
+    g = torch.Generator(device="cuda").manual_seed(n + rows)
+    z = -30.0 + 1e-3 * torch.rand(rows, n, generator=g, device="cuda")
+    z[torch.arange(rows, device="cuda"), torch.randint(0, n, (rows,), generator=g, device="cuda")] = 0.0
+    u = torch.rand(rows, generator=g, device="cuda", dtype=torch.float64)
+    check_draw(P, z, u, temperature=40.0, top_k=n // 2)
+    check_draw(P, z, u, temperature=40.0, top_p=0.6)
+    check_draw(P, z, u, temperature=40.0, top_k=n - 5, top_p=0.3, min_p=0.2)
+
+
 @pytest.mark.parametrize("n", [3, 300, 3000, 20000])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
 def test_draw_masks(P, n, dtype):
@@ -523,3 +547,66 @@ def test_posterior_predictive_of_a_chain(P):
     check = P.draw(z, u, 0.9, 100, 0.95)
     assert torch.equal(index, check[0]) and torch.equal(logp, check[1])
     check_draw(P, z, u, 0.9, 100, 0.95)
+
+
+def test_product_in_parts(P):
+    """More rows than a launch has threads for: the last part, and both sides of the borders."""
+    rows = (1 << 28) + 70
+    g = torch.Generator(device="cuda").manual_seed(5)
+    x = torch.rand(rows, 1, generator=g, device="cuda", dtype=torch.bfloat16)
+    w = P.quantize(torch.randn(2, 1, generator=g, device="cuda"))
+    out = P.product(x, w, torch.bfloat16)
+    for i in (0, 1 << 27, 1 << 28, rows):
+        part = slice(max(0, i - 100), min(rows, i + 100))
+        want = values(P.quantize(x[part])) @ values(w).T
+        assert torch.equal(out[part].double(), want.to(torch.bfloat16).double())  # one product a value, rounded once
+    last = x.t()[:, -300:].t()
+    assert torch.equal(P.product(last, w, torch.bfloat16), out[-300:])
+
+
+@pytest.mark.parametrize("rows,n", [((1 << 20) + 70, 3), (16500, 8200)])
+def test_draw_in_parts(P, rows, n):
+    g = torch.Generator(device="cuda").manual_seed(n)
+    z = torch.randn(rows, n, generator=g, device="cuda", dtype=torch.bfloat16)
+    u = torch.rand(rows, generator=g, device="cuda")
+    each = dict(temperature=0.5 + torch.rand(rows, generator=g, device="cuda"), top_k=torch.randint(1, n, (rows,), generator=g, device="cuda", dtype=torch.int32),
+                top_p=torch.rand(rows, generator=g, device="cuda"), min_p=0.01 * torch.rand(rows, generator=g, device="cuda"))
+    column, logp = P.draw(z, u, **each)
+    border = (1 << 20) if n == 3 else (1 << 27) // n
+    for part in (slice(0, 40), slice(border - 40, border + 40), slice(rows - 40, rows)):
+        few = {k: v[part] for k, v in each.items()}
+        check_draw(P, z[part], u[part], **few)
+        want = P.draw(z[part], u[part], **few)
+        assert torch.equal(column[part], want[0]) and torch.allclose(logp[part], want[1], rtol=2.0 ** -22, atol=1e-12)  # sums of another shape
+
+
+def test_threads_at_once(P):
+    """Four threads, each on a stream of its own."""
+    import threading
+
+    g = torch.Generator(device="cuda").manual_seed(8)
+    sets = []
+    for i in range(4):
+        x = torch.randn(90 + 200 * i, 300, generator=g, device="cuda")
+        w = P.quantize(torch.randn(700 + i, 300, generator=g, device="cuda"))
+        z = torch.randn(5, 9000 + i, generator=g, device="cuda")
+        u = torch.rand(5, generator=g, device="cuda")
+        sets.append((x, w, z, u, P.product(x, w), P.draw(z, u, top_p=0.8)))
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(x, w, z, u, product, drawn):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            for _ in range(20):
+                a, b = P.product(x, w), P.draw(z, u, top_p=0.8)
+                stream.synchronize()
+                if not (torch.equal(a, product) and torch.equal(b[0], drawn[0]) and torch.equal(b[1], drawn[1])):
+                    wrong.append(x.shape)
+
+    threads = [threading.Thread(target=work, args=s) for s in sets]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
