@@ -14,8 +14,8 @@
 //
 // u is compared with sums of up to n weights, so weights and sums are double: with float sums a draw among 1e5 weights
 // would land in a neighbouring column once in a few hundred draws.  Sums that pick a border are taken in 64-bit whole
-// numbers (weights to 2^-63 n), so that the order of atomic additions does not matter; the sums u is compared with have
-// a fixed shape.
+// numbers (weights to 2^-51, or 2^-63 n if that is more), so that the order of atomic additions does not matter; the
+// sums u is compared with have a fixed shape.
 #pragma once
 
 #include "mhlik_predict.hpp"
@@ -137,7 +137,14 @@ template <int BINS> struct DrawBin {
   }
 };
 
-__device__ __forceinline__ unsigned long long draw_fixed(double w, int shift) { return (unsigned long long)rint(ldexp(w, shift)); }
+// rint(w 2^shift) of a weight, shift <= 51: added to 2^(52 - shift), its whole multiples of 2^-shift are the low bits of
+// the sum.  Two instructions, where scaling and converting takes twelve.
+__device__ __forceinline__ unsigned long long draw_fixed(double w, int shift)
+{
+  const int one = (1023 + 52 - shift) << 20;
+  const double v = w + __hiloint2double(one, 0);
+  return (unsigned long long)(uint32_t)(__double2hiint(v) - one) << 32 | (uint32_t)__double2loint(v);
+}
 
 // Position in the order: smaller is earlier (larger value, lower column).
 __device__ __forceinline__ unsigned long long draw_place(float z, int j)
@@ -178,21 +185,17 @@ __device__ int draw_pick(const double (&w)[VPT], double aim, double *total, doub
   int place = -1;
   if (wave == pick) {
     aim -= before;
-    int at = -1;
-    double sum = 0.0, done_before = 0.0, mine = 0.0;
-    bool done = false;
+    int at = 0;
+    double mine = w[0];
+    if (VPT > 1) { // the same for the runs of 64: lane i has the sum of run i
+      const double each = wave_sums<VPT>(w), to = wave_running(each);
+      const unsigned long long runs = (1ull << VPT) - 1, over = __ballot(each > 0.0 && to > aim) & runs, some = __ballot(each > 0.0) & runs;
+      at = over ? __ffsll(over) - 1 : 63 - __clzll((long long)some);
+      if (at > 0) aim -= wave_lane(to, at - 1);
 #pragma unroll
-    for (int i = 0; i < VPT; i++) { // the same for the runs of 64
-      const double v = wave_sum(w[i]);
-      if (!done && v > 0.0) {
-        at = i;
-        done_before = sum;
-        mine = w[i];
-        done = sum + v > aim;
-      }
-      sum += v;
+      for (int i = 1; i < VPT; i++)
+        if (i == at) mine = w[i];
     }
-    aim -= done_before;
     const double run = wave_running(mine);
     const unsigned long long over = __ballot(mine > 0.0 && run > aim), some = __ballot(mine > 0.0);
     const int who = over ? __ffsll(over) - 1 : 63 - __clzll((long long)some);
@@ -274,7 +277,7 @@ __device__ void draw_narrow(DrawRow<T> &r, DrawShared &s, int shift, uint32_t k,
       const uint32_t bin = (key >> low) & 255u;
       atomicAdd(&s.count[bin], 1u);
       if (BY_MASS) {
-        const unsigned long long m = (unsigned long long)rint(ldexp(draw_weight(z, r.max, r.rate), shift));
+        const unsigned long long m = draw_fixed(draw_weight(z, r.max, r.rate), shift);
         if (m) atomicAdd(&s.mass[bin], m);
       }
     }
@@ -400,10 +403,10 @@ template <int THREADS> struct ShortShared {
 };
 
 // The place of the k-th of the values above -inf; unchanged if there are no more than k.  False: no room.
-template <int THREADS, int VPT, int BINS, typename AT>
-__device__ bool draw_by_count(const float (&z)[VPT], AT at, const DrawBin<BINS> &bin, uint32_t k, ShortShared<THREADS> &s, DrawEnd *end)
+template <int THREADS, int VPT, typename AT>
+__device__ bool draw_by_count(const float (&z)[VPT], const int (&bin)[VPT], AT at, uint32_t k, ShortShared<THREADS> &s, DrawEnd *end)
 {
-  constexpr int kRun = BINS / THREADS;
+  constexpr int kRun = ShortShared<THREADS>::kBins / THREADS;
   const int tid = threadIdx.x;
 #pragma unroll
   for (int i = 0; i < kRun; i++) s.count[tid + i * THREADS] = 0;
@@ -411,7 +414,7 @@ __device__ bool draw_by_count(const float (&z)[VPT], AT at, const DrawBin<BINS> 
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < VPT; i++)
-    if (z[i] > -HUGE_VALF) atomicAdd(&s.count[bin.of(z[i])], 1u);
+    if (z[i] > -HUGE_VALF) atomicAdd(&s.count[bin[i]], 1u);
   __syncthreads();
   uint32_t here[kRun], mine = 0, all;
 #pragma unroll
@@ -430,7 +433,7 @@ __device__ bool draw_by_count(const float (&z)[VPT], AT at, const DrawBin<BINS> 
   const int border = (int)s.i[31];
 #pragma unroll
   for (int i = 0; i < VPT; i++)
-    if (z[i] > -HUGE_VALF && bin.of(z[i]) == border) {
+    if (z[i] > -HUGE_VALF && bin[i] == border) {
       const uint32_t q = atomicAdd(&s.i[30], 1u);
       if (q < ShortShared<THREADS>::kCap) s.place[q] = draw_place(z[i], at(i));
     }
@@ -448,13 +451,13 @@ __device__ bool draw_by_count(const float (&z)[VPT], AT at, const DrawBin<BINS> 
   return true;
 }
 
-// Of the values up to end->place, the place of the last before which (with `base` before them all) less than the target
+// Of the values with a weight, the place of the last before which (with `base` before them all) less than the target
 // lies; share: the target is this share of their mass.  False: no room.
-template <int THREADS, int VPT, int BINS, typename AT>
-__device__ bool draw_by_mass(const float (&z)[VPT], const double (&weight)[VPT], AT at, const DrawBin<BINS> &bin, unsigned long long base,
+template <int THREADS, int VPT, typename AT>
+__device__ bool draw_by_mass(const float (&z)[VPT], const double (&weight)[VPT], const int (&bin)[VPT], AT at, unsigned long long base,
                              double share, double target, int shift, ShortShared<THREADS> &s, DrawEnd *end)
 {
-  constexpr int kRun = BINS / THREADS;
+  constexpr int kBins = ShortShared<THREADS>::kBins, kRun = kBins / THREADS;
   const int tid = threadIdx.x;
   const double unit = ldexp(1.0, -shift);
   __syncthreads();
@@ -462,15 +465,14 @@ __device__ bool draw_by_mass(const float (&z)[VPT], const double (&weight)[VPT],
   for (int i = 0; i < kRun; i++) s.mass[tid + i * THREADS] = 0;
   if (tid == 0) {
     s.i[30] = 0;
-    s.i[31] = BINS;
+    s.i[31] = kBins;
   }
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < VPT; i++)
-    if (weight[i] > 0.0 && end->kept(z[i], at(i))) {
-      const unsigned long long m = draw_fixed(weight[i], shift);
-      if (m) atomicAdd(&s.mass[bin.of(z[i])], m);
-    }
+  for (int i = 0; i < VPT; i++) {
+    const unsigned long long m = draw_fixed(weight[i], shift);
+    if (m) atomicAdd(&s.mass[bin[i]], m);
+  }
   __syncthreads();
   unsigned long long here[kRun], mine = 0, all;
 #pragma unroll
@@ -488,10 +490,10 @@ __device__ bool draw_by_mass(const float (&z)[VPT], const double (&weight)[VPT],
   if (tid == 0) s.q[31] = 0;
   __syncthreads();
   const int border = (int)s.i[31];
-  if (border == BINS) return true; // what is here ends before the target: all of it
+  if (border == kBins) return true; // what is here ends before the target: all of it
 #pragma unroll
   for (int i = 0; i < VPT; i++)
-    if (weight[i] > 0.0 && end->kept(z[i], at(i)) && bin.of(z[i]) == border) {
+    if (weight[i] > 0.0 && bin[i] == border) {
       const uint32_t q = atomicAdd(&s.i[30], 1u);
       if (q < ShortShared<THREADS>::kCap) {
         s.place[q] = draw_place(z[i], at(i));
@@ -517,15 +519,34 @@ __device__ bool draw_by_mass(const float (&z)[VPT], const double (&weight)[VPT],
   return true;
 }
 
-// Narrows the kept prefix by the row's top-k and top-p.  z: -inf where there is nothing; column j of z[i] from at(i);
-// weight: of z[i].  False if a border's bin holds more values than there is room for.
+// Weights behind the end of the kept prefix become 0.
+template <int VPT, typename AT> __device__ __forceinline__ void draw_cut(const float (&z)[VPT], double (&weight)[VPT], AT at, const DrawEnd &end)
+{
+#pragma unroll
+  for (int i = 0; i < VPT; i++)
+    if (!end.kept(z[i], at(i))) weight[i] = 0.0;
+}
+
+// Cuts the row's top-k and top-p.  z: -inf where there is nothing; column j of z[i] from at(i); weight: of z[i].  False if
+// a border's bin holds more values than there is room for.
 template <int THREADS, int VPT, typename AT>
-__device__ bool draw_short_narrow(const float (&z)[VPT], const double (&weight)[VPT], AT at, float max, float min, const DrawChoice &c,
-                                  int shift, ShortShared<THREADS> &s, DrawEnd *end)
+__device__ bool draw_short_narrow(const float (&z)[VPT], double (&weight)[VPT], AT at, float max, float min, const DrawChoice &c,
+                                  int shift, ShortShared<THREADS> &s)
 {
   const DrawBin<ShortShared<THREADS>::kBins> bin(max, min, c.temp);
-  if (c.k && !draw_by_count<THREADS, VPT>(z, at, bin, (uint32_t)c.k, s, end)) return false;
-  return c.share >= 1.0 || draw_by_mass<THREADS, VPT>(z, weight, at, bin, 0, c.share, 0.0, shift, s, end);
+  int bins[VPT];
+#pragma unroll
+  for (int i = 0; i < VPT; i++) bins[i] = bin.of(z[i]);
+  DrawEnd end{~0ull};
+  if (c.k) {
+    if (!draw_by_count<THREADS, VPT>(z, bins, at, (uint32_t)c.k, s, &end)) return false;
+    draw_cut<VPT>(z, weight, at, end);
+  }
+  if (c.share < 1.0) {
+    if (!draw_by_mass<THREADS, VPT>(z, weight, bins, at, 0, c.share, 0.0, shift, s, &end)) return false;
+    draw_cut<VPT>(z, weight, at, end);
+  }
+  return true;
 }
 
 // What the kernels that finish a row keep in LDS: one of the two at a time.
@@ -570,7 +591,7 @@ template <typename T, int THREADS, int VPT> __global__ __launch_bounds__(THREADS
     nan |= v != v;
     z[i] = draw_finite(v);
     max = fmaxf(max, z[i]);
-    if (z[i] > -HUGE_VALF) min = fminf(min, z[i]);
+    min = fminf(min, z[i] > -HUGE_VALF ? z[i] : HUGE_VALF);
   }
   const DrawChoice c = draw_choice(a, row);
   max = wave_max(max);
@@ -609,12 +630,12 @@ template <typename T, int THREADS, int VPT> __global__ __launch_bounds__(THREADS
   double w[VPT];
 #pragma unroll
   for (int i = 0; i < VPT; i++) w[i] = draw_weight(z[i], max, c.rate);
-  DrawEnd end{~0ull};
   if (c.k || c.share < 1.0)
-    if (!draw_short_narrow<THREADS, VPT>(z, w, at, max, min, c, shift, s.quick, &end)) end = draw_whole<T, THREADS>(a, row, c, max, shift, s.whole);
+    if (!draw_short_narrow<THREADS, VPT>(z, w, at, max, min, c, shift, s.quick))
+      draw_cut<VPT>(z, w, at, draw_whole<T, THREADS>(a, row, c, max, shift, s.whole)); // (after a cut by top-k the same end, or an earlier one)
 #pragma unroll
   for (int i = 0; i < VPT; i++)
-    if (!end.kept(z[i], at(i)) || w[i] < c.least) w[i] = 0.0;
+    if (w[i] < c.least) w[i] = 0.0;
   double total, weight, rest;
   __syncthreads();
   const int place = draw_pick<THREADS, VPT, true>(w, c.u, &total, &weight, &rest, s.quick.d);
@@ -972,10 +993,10 @@ template <typename T, int VPT> __global__ __launch_bounds__(1024) void draw_fini
       z[i] = place_of(i) < listed ? list[place_of(i)].z : -HUGE_VALF;
       w[i] = draw_weight(z[i], max, c.rate);
     }
-    if (kind == kRowList && draw_short_narrow<kThreads, kList>(z, w, at, max, min, c, shift, s.quick, &end)) {
+    if (kind == kRowList && draw_short_narrow<kThreads, kList>(z, w, at, max, min, c, shift, s.quick)) {
 #pragma unroll
       for (int i = 0; i < kList; i++)
-        if (!end.kept(z[i], at(i)) || w[i] < c.least) w[i] = 0.0;
+        if (w[i] < c.least) w[i] = 0.0;
       double total, weight, rest;
       __syncthreads();
       const int place = draw_pick<kThreads, kList, true>(w, c.u, &total, &weight, &rest, s.quick.d);
@@ -1002,7 +1023,10 @@ template <typename T, int VPT> __global__ __launch_bounds__(1024) void draw_fini
         low = fminf(low, s.quick.g[q]);
       }
       const DrawBin<ShortShared<kThreads>::kBins> bin(top, low, HUGE_VAL);
-      whole = !draw_by_mass<kThreads, kList>(z, w, at, bin, cell.above, -1.0, cell.target, shift, s.quick, &end);
+      int bins[kList];
+#pragma unroll
+      for (int i = 0; i < kList; i++) bins[i] = bin.of(z[i]);
+      whole = !draw_by_mass<kThreads, kList>(z, w, bins, at, cell.above, -1.0, cell.target, shift, s.quick, &end);
       if (whole) end.place = ~0ull;
     } else
       whole = true;

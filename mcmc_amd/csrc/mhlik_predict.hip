@@ -305,7 +305,7 @@ template <typename T> int draw_part(const DrawArgs &a, const DrawPlan &p, int sh
 
 template <typename T> int draw_launch(DrawArgs a, const DrawPlan &p, hipStream_t stream)
 {
-  int shift = 63; // weights in whole numbers: n of them stay below 2^63
+  int shift = 51; // weights in whole numbers: n of them stay below 2^63
   while (((int64_t)1 << (63 - shift)) < a.n) shift--;
   for (int64_t left = a.rows; left > 0; left -= p.part) {
     const int64_t rows = a.rows = std::min(left, p.part);

@@ -1,6 +1,8 @@
 // mhlik_predict.hpp -- what the kernels of the predictive operators share (mhlik_q8.hpp, mhlik_draw.hpp).
 #pragma once
 
+#include <type_traits>
+
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -68,6 +70,42 @@ __device__ __forceinline__ double wave_lane(double v, int from)
 template <typename V> __device__ __forceinline__ V wave_running(V v)
 {
   return wave_scan(v, (V)0, [](V a, V b) { return a + b; });
+}
+// Sums over the wave of N values a lane has, N a power of two up to 16: lane l gets that of value l % N.  While there are
+// several values, lanes give half of them to a partner and add up the other half: N - 1 exchanges and 6 - log2 N more,
+// not 6 N.
+template <int N> __device__ __forceinline__ double wave_sums(const double (&w)[N])
+{
+#if defined(__HIP_DEVICE_COMPILE__)
+  const int lane = threadIdx.x % kWave;
+  double v[N];
+#pragma unroll
+  for (int i = 0; i < N; i++) v[i] = w[i];
+  auto halve = [&](auto n, auto from) { // the partner agrees in the bits above n, and differs in n (and below, where nothing is decided)
+#pragma unroll
+    for (int i = 0; i < n.value; i++) {
+      const bool upper = lane & n.value;
+      v[i] = (upper ? v[i + n.value] : v[i]) + from(upper ? v[i] : v[i + n.value]);
+    }
+  };
+  if constexpr (N >= 16) halve(std::integral_constant<int, 8>{}, [](double x) { return dpp_move<0x140, 0xf>(x, 0.0); }); // lane ^ 15
+  if constexpr (N >= 8) halve(std::integral_constant<int, 4>{}, [](double x) { return dpp_move<0x141, 0xf>(x, 0.0); });  // lane ^ 7
+  if constexpr (N >= 4) halve(std::integral_constant<int, 2>{}, [](double x) { return dpp_move<0x4e, 0xf>(x, 0.0); });   // lane ^ 2
+  if constexpr (N >= 2) halve(std::integral_constant<int, 1>{}, [](double x) { return dpp_move<0xb1, 0xf>(x, 0.0); });   // lane ^ 1
+  double s = v[0];
+  if constexpr (N < 2) s += dpp_move<0xb1, 0xf>(s, 0.0);
+  if constexpr (N < 4) s += dpp_move<0x4e, 0xf>(s, 0.0);
+  if constexpr (N < 8) s += dpp_move<0x124, 0xf>(s, 0.0);  // four lanes round in the 16
+  if constexpr (N < 16) s += dpp_move<0x128, 0xf>(s, 0.0); // eight
+  auto swapped = [](double x, auto swap) { // what two rows of 16, or two halves, have, added up in both
+    const auto lo = swap((unsigned)__double2loint(x)), hi = swap((unsigned)__double2hiint(x));
+    return __hiloint2double((int)hi[0], (int)lo[0]) + __hiloint2double((int)hi[1], (int)lo[1]);
+  };
+  s = swapped(s, [](unsigned x) { return __builtin_amdgcn_permlane16_swap(x, x, false, false); });
+  return swapped(s, [](unsigned x) { return __builtin_amdgcn_permlane32_swap(x, x, false, false); });
+#else
+  return w[0];
+#endif
 }
 template <typename V> __device__ __forceinline__ V wave_sum(V v) { return wave_last(wave_running(v)); }
 __device__ __forceinline__ float wave_max(float v)
