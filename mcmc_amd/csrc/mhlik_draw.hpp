@@ -692,11 +692,13 @@ struct LongSpace {
 // What a row needs.
 __device__ inline int draw_kind(const DrawChoice &c, bool bad, float max)
 {
-  if (bad || c.bad || max == -HUGE_VALF) return kRowNothing;
-  if (c.greedy) return kRowGreedy;
-  if (c.k) return kRowList;
-  if (c.share < 1.0) return kRowNucleus;
-  return c.least > 0.0 ? kRowSums : kRowPlain;
+  const int kind = bad || c.bad || max == -HUGE_VALF ? kRowNothing
+                   : c.greedy                        ? kRowGreedy
+                   : c.k                             ? kRowList
+                   : c.share < 1.0                   ? kRowNucleus
+                   : c.least > 0.0                   ? kRowSums
+                                                     : kRowPlain;
+  return __builtin_amdgcn_readfirstlane(kind); // all lanes have the same
 }
 
 // The row's largest and smallest value from its units'; every wave does it for itself.
@@ -787,6 +789,9 @@ __global__ __launch_bounds__(kBlock) void draw_top_kernel(DrawArgs a, LongSpace 
   if (lane == 0) g.part[row * g.units + unit] = LongPart{max, min, first, any, mass};
 }
 
+// Weights that are worked out together, not each in a branch of its own: one is a chain of 17 steps.
+constexpr int kAtOnce = 8;
+
 template <typename T, int VEC, int VPT>
 __global__ __launch_bounds__(kBlock) void draw_histo_kernel(DrawArgs a, LongSpace g, int groups, int shift)
 {
@@ -807,12 +812,21 @@ __global__ __launch_bounds__(kBlock) void draw_histo_kernel(DrawArgs a, LongSpac
   __syncthreads();
   const DrawBin<kLongBins> bin(max, min, c.temp);
   while (unit < g.units) {
+    if (kind == kRowList) {
 #pragma unroll
-    for (int i = 0; i < VPT; i++)
-      if (z[i] > -HUGE_VALF) {
-        const unsigned long long m = kind == kRowList ? 1 : draw_fixed(draw_weight(z[i], max, c.rate), shift);
-        if (m) atomicAdd(&bins[bin.of(z[i])], m);
+      for (int i = 0; i < VPT; i++)
+        if (z[i] > -HUGE_VALF) atomicAdd(&bins[bin.of(z[i])], 1ull);
+    } else {
+#pragma unroll
+      for (int o = 0; o < VPT; o += kAtOnce) {
+        unsigned long long m[kAtOnce];
+#pragma unroll
+        for (int i = 0; i < kAtOnce; i++) m[i] = draw_fixed(draw_weight(z[o + i], max, c.rate), shift);
+#pragma unroll
+        for (int i = 0; i < kAtOnce; i++)
+          if (m[i]) atomicAdd(&bins[bin.of(z[o + i])], m[i]);
       }
+    }
     unit += groups * 4;
     if (unit < g.units) draw_load<T, VEC, VPT>(zp, (int)a.n, unit * VPT * kWave, z);
   }
@@ -870,8 +884,8 @@ __global__ __launch_bounds__(kBlock) void draw_collect_kernel(DrawArgs a, LongSp
     }
     if (kind == kRowList && tid == 0 && all < (unsigned long long)c.k) cell.too_long = all > kLongList; // fewer values than k: all
     __syncthreads();
-    border = cell.bin;
-    too_long = cell.too_long;
+    border = __builtin_amdgcn_readfirstlane(cell.bin);
+    too_long = __builtin_amdgcn_readfirstlane(cell.too_long) != 0;
     if (group == 0 && tid == 0) g.cell[row] = cell;
   }
   if (u >= g.units || too_long) return;
@@ -881,27 +895,27 @@ __global__ __launch_bounds__(kBlock) void draw_collect_kernel(DrawArgs a, LongSp
   LongCand *list = g.list + (row * g.units + u) * (kUnit / 2);
 #pragma unroll
   for (int v = 0; v < VPT / VEC; v++) {
+    int b[VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; e++) b[e] = bin.of(z[v * VEC + e]);
+    if (kind != kRowList) { // (no branch for each: a weight is a chain of 17 steps)
+#pragma unroll
+      for (int e = 0; e < VEC; e++) {
+        const double w = draw_weight(z[v * VEC + e], max, c.rate);
+        kept += (kind == kRowSums || b[e] < border) && w >= c.least ? w : 0.0;
+      }
+    }
+    if (kind == kRowSums) continue;
     bool take[VEC];
     int earlier = 0, total = 0; // of the same columns in lower lanes; of all lanes
 #pragma unroll
     for (int e = 0; e < VEC; e++) {
-      const float x = z[v * VEC + e];
-      take[e] = false;
-      if (kind == kRowSums) {
-        const double w = draw_weight(x, max, c.rate);
-        if (w >= c.least) kept += w;
-      } else if (x > -HUGE_VALF) {
-        const int b = bin.of(x);
-        take[e] = kind == kRowList ? b <= border : b == border;
-        if (kind == kRowNucleus && b < border) {
-          const double w = draw_weight(x, max, c.rate);
-          if (w >= c.least) kept += w;
-        }
-      }
+      take[e] = z[v * VEC + e] > -HUGE_VALF && (kind == kRowList ? b[e] <= border : b[e] == border);
       const unsigned long long t = __ballot(take[e]);
-      earlier += __popcll(t & ((1ull << lane) - 1));
+      earlier = (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(t >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)t, (uint32_t)earlier));
       total += __popcll(t);
     }
+    if (total == 0) continue;
 #pragma unroll
     for (int e = 0; e < VEC; e++)
       if (take[e]) {

@@ -220,7 +220,7 @@ struct DrawPlan {
 };
 
 constexpr int kShortMax = 8192;  // columns that fit a workgroup's registers (1024 threads, 8 each)
-constexpr int64_t kLongVpt = 32; // a unit: 2048 columns; 512 where those would leave the chip's 1024 SIMDs idle
+constexpr int64_t kLongVpt = 32; // a unit: 2048 columns; 1024 where those would not give the 1024 SIMDs two each
 
 DrawPlan draw_plan(int64_t rows, int64_t n, void *workspace)
 {
@@ -229,7 +229,7 @@ DrawPlan draw_plan(int64_t rows, int64_t n, void *workspace)
   p.part = kPartDrawRows;
   if (p.short_rows) return p;
   if (n <= kLongVpt * kWave * kLongUnits) rows = p.part = std::min(rows, std::max<int64_t>(1, kPartWeights / n));
-  p.vpt = rows * ((n + kLongVpt * kWave - 1) / (kLongVpt * kWave)) < 2048 && n <= (int64_t)8 * kWave * kLongUnits ? 8 : kLongVpt;
+  p.vpt = rows * ((n + kLongVpt * kWave - 1) / (kLongVpt * kWave)) < 2048 && n <= (int64_t)16 * kWave * kLongUnits ? 16 : kLongVpt;
   const int64_t unit = p.vpt * kWave, units = (n + unit - 1) / unit;
   if (units > kLongUnits) {
     p.vpt = 0;
@@ -294,8 +294,8 @@ template <typename T> int draw_part(const DrawArgs &a, const DrawPlan &p, int sh
     const bool histo = a.top_k || a.top_p || (a.top_k_all > 0 && a.top_k_all < a.n) || a.top_p_all < 1.0;
     const bool collect = histo || a.min_p || a.min_p_all > 0.0;
     constexpr int kVec = 16 / sizeof(T);
-    if (p.vpt == 8)
-      draw_long<T, kVec, 8>(a, p.space, shift, histo, collect, stream);
+    if (p.vpt == 16)
+      draw_long<T, kVec, 16>(a, p.space, shift, histo, collect, stream);
     else
       draw_long<T, kVec, kLongVpt>(a, p.space, shift, histo, collect, stream);
   }
