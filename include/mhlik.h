@@ -451,7 +451,7 @@ enum { MHLIK_T_Q8 = 0, MHLIK_T_F64 = 1, MHLIK_T_F32 = 2, MHLIK_T_BF16 = 3, MHLIK
  *   data [i][128 b + c] = e4m3(x 2^-k)   (to nearest even, from the exact quotient)
  *   scale[i][b]         = k + 127,       k the least integer in [-96, 119] with |x| <= 448 2^k for the block's finite x
  * data has 128 ceil(cols/128) bytes a row (columns past the last: 0), starts at a multiple of 16 bytes; scale has
- * 4 ceil(cols/512) bytes a row (spare ones: 127).  Values that are not finite, or exceed 448 2^119, become NaN.
+ * 4 ceil(cols/512) bytes a row (spare ones: 127), starts at a multiple of 4.  Values that are not finite, or exceed 448 2^119, become NaN.
  * x[i * row_stride + c * col_stride], of any type but MHLIK_T_Q8; strides count elements and are not negative.
  * 0 <= rows <= 2^40, 1 <= cols <= 2^22.  Rows made elsewhere: scale bytes 31 .. 246, as these k have. */
 int mhlik_q8_quantize(const void *x, int32_t type, int64_t rows, int64_t cols, int64_t row_stride, int64_t col_stride,

@@ -66,6 +66,7 @@ int check_rows8(const char *what, const void *data, const void *scale, int64_t r
 {
   if (rows && (!data || !scale)) return fail_no_ctx(MHLIK_EINVAL, "%s: data and scale must not be NULL", what);
   if (!aligned16(data)) return fail_no_ctx(MHLIK_EINVAL, "%s: data must start at a multiple of 16 bytes", what);
+  if ((uintptr_t)scale & 3) return fail_no_ctx(MHLIK_EINVAL, "%s: scale must start at a multiple of 4 bytes", what);
   return MHLIK_OK;
 }
 

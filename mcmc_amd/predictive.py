@@ -71,6 +71,7 @@ class Block8:
             raise ValueError("scale has shape %s; wanted %s" % (tuple(scale.shape), (rows, (blocks + 3) // 4 * 4)))
         _need(data.is_contiguous() and scale.is_contiguous(), "data and scale must be contiguous")
         _need(data.data_ptr() % 16 == 0, "data must start at a multiple of 16 bytes")
+        _need(scale.data_ptr() % 4 == 0, "scale must start at a multiple of 4 bytes")
         self.data, self.scale, self.cols, self.rows, self.device = data, scale, int(cols), rows, device
 
     def dequantize(self):

@@ -28,7 +28,7 @@ def _refused(lib, rc, text):
     (dict(cols=0), "1 <= cols"), (dict(cols=(1 << 22) + 1), "1 <= cols"), (dict(rows=(1 << 40) + 1), "0 <= rows"),
     (dict(x=None), "x must not be NULL"), (dict(x=FAKE + 2), "not aligned to its type"), (dict(rs=-1), "strides must not be negative"),
     (dict(cs=-4), "strides must not be negative"), (dict(data=None), "must not be NULL"), (dict(scale=None), "must not be NULL"),
-    (dict(data=FAKE + 8), "multiple of 16 bytes"),
+    (dict(data=FAKE + 8), "multiple of 16 bytes"), (dict(scale=FAKE + 2), "multiple of 4 bytes"),
 ])
 def test_quantize_refuses(lib, change, text):
     a = dict(x=FAKE, type=2, rows=4, cols=100, rs=100, cs=1, data=FAKE, scale=FAKE)
@@ -57,6 +57,7 @@ def _operands(**change):
     (dict(x_type=2, x=FAKE + 1), "not aligned to its type"),
     (dict(x_type=2), "workspace"), (dict(x_type=2, workspace=FAKE, workspace_bytes=100 * (384 + 4) - 1), "workspace"),
     (dict(x_type=2, workspace=FAKE + 8, workspace_bytes=1 << 20), "workspace"),
+    (dict(x_scale=FAKE + 1), "x: scale must start"), (dict(w_scale=FAKE + 2), "w: scale must start"),
 ])
 def test_product_refuses(lib, change, text):
     rc = lib.mhlik_q8_product(C.byref(_operands(**change)), -1, None)
