@@ -78,7 +78,7 @@ class Block8:
         """The values the rows stand for, as float32 [rows, cols]."""
         blocks = self.data.shape[1] // BLOCK
         step = torch.ldexp(torch.ones((), device=self.device), self.scale[:, :blocks].int() - 127)
-        return (self.data.float().view(-1, blocks, BLOCK) * step[:, :, None]).view(self.data.shape)[:, : self.cols]
+        return (self.data.float().view(self.rows, blocks, BLOCK) * step[:, :, None]).view(self.data.shape)[:, : self.cols]
 
 
 def quantize(x):
@@ -256,6 +256,9 @@ class PosteriorPredictive:
         _same("u", _given("u", u, 1, _U), x.device)
         _need(u.shape[0] == rows, "u has %d values for %d rows", u.shape[0], rows)
         choices = {"temperature": temperature, "top_k": top_k, "top_p": top_p, "min_p": min_p}
+        for name, value in choices.items():
+            if isinstance(value, torch.Tensor):
+                _each(name, value, _I32 if name == "top_k" else _F32, rows, x.device)
         index = torch.empty(rows, dtype=torch.int64, device=x.device)
         logp = torch.empty(rows, dtype=torch.float32, device=x.device)
         zero = torch.zeros((), device=x.device)

@@ -547,6 +547,27 @@ def test_posterior_predictive_of_a_chain(P):
     check = P.draw(z, u, 0.9, 100, 0.95)
     assert torch.equal(index, check[0]) and torch.equal(logp, check[1])
     check_draw(P, z, u, 0.9, 100, 0.95)
+    each = torch.linspace(0.5, 1.5, 200, device="cuda")
+    index, logp = pp.case_deletion(x, u, each)
+    check = P.draw(z, u, each)
+    assert torch.equal(index, check[0]) and torch.equal(logp, check[1])
+    for rows in (199, 201):  # one choice a row, neither fewer nor more
+        with pytest.raises(ValueError, match="temperature has %d values for 200 rows" % rows):
+            pp.case_deletion(x, u, torch.ones(rows, device="cuda"))
+    with pytest.raises(ValueError, match="u has 201 values for 200 rows"):
+        pp.case_deletion(x, torch.rand(201, device="cuda"))
+
+
+def test_no_rows(P):
+    x = torch.zeros(0, 300, device="cuda")
+    q = P.quantize(x)
+    assert q.dequantize().shape == (0, 300)
+    w = P.quantize(torch.ones(4, 300, device="cuda"))
+    assert P.product(q, w).shape == (0, 4) and P.product(w, q).shape == (4, 0)
+    index, logp = P.draw(torch.zeros(0, 9000, device="cuda"), torch.zeros(0, device="cuda"))
+    assert index.shape == (0,) and logp.shape == (0,)
+    pp = P.PosteriorPredictive(torch.ones(4, 300, device="cuda"))
+    assert pp.probability(x).shape == (0,) and pp.case_deletion(x, torch.zeros(0, device="cuda"))[0].shape == (0,)
 
 
 def test_product_in_parts(P):
