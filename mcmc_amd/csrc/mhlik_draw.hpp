@@ -152,6 +152,16 @@ __device__ __forceinline__ unsigned long long draw_place(float z, int j)
   return (unsigned long long)~draw_key(z) << 32 | (uint32_t)j;
 }
 
+// The same value, of which the compiler does not know that it is: what was worked out from it before is worked out again,
+// and need not wait in a register.
+template <typename V> __device__ __forceinline__ V draw_again(V v)
+{
+#if defined(__HIP_DEVICE_COMPILE__)
+  asm volatile("" : "+v"(v));
+#endif
+  return v;
+}
+
 // The kept prefix ends with this place.
 struct DrawEnd {
   unsigned long long place;
@@ -393,7 +403,8 @@ template <int THREADS> struct ShortShared {
   static constexpr int kBins = THREADS < 256 ? 256 : THREADS;          // one a thread, or four
   static constexpr int kCap = THREADS < 256 ? 128 : THREADS;           // values of a border's bin
   unsigned long long mass[kBins];
-  uint32_t count[kBins];
+  uint32_t count[kBins];               // later the columns of what top-k left
+  float value[THREADS];                // ... and their values
   unsigned long long place[kCap];
   unsigned long long cmass[kCap];
   double d[32];
@@ -435,7 +446,7 @@ __device__ bool draw_by_count(const float (&z)[VPT], const int (&bin)[VPT], AT a
   for (int i = 0; i < VPT; i++)
     if (z[i] > -HUGE_VALF && bin[i] == border) {
       const uint32_t q = atomicAdd(&s.i[30], 1u);
-      if (q < ShortShared<THREADS>::kCap) s.place[q] = draw_place(z[i], at(i));
+      if (q < ShortShared<THREADS>::kCap) s.place[q] = draw_place(draw_again(z[i]), at(i));
     }
   __syncthreads();
   const int m = (int)s.i[30];
@@ -496,8 +507,8 @@ __device__ bool draw_by_mass(const float (&z)[VPT], const double (&weight)[VPT],
     if (weight[i] > 0.0 && bin[i] == border) {
       const uint32_t q = atomicAdd(&s.i[30], 1u);
       if (q < ShortShared<THREADS>::kCap) {
-        s.place[q] = draw_place(z[i], at(i));
-        s.cmass[q] = draw_fixed(weight[i], shift);
+        s.place[q] = draw_place(draw_again(z[i]), at(i));
+        s.cmass[q] = draw_fixed(draw_again(weight[i]), shift);
       }
     }
   __syncthreads();
@@ -524,7 +535,7 @@ template <int VPT, typename AT> __device__ __forceinline__ void draw_cut(const f
 {
 #pragma unroll
   for (int i = 0; i < VPT; i++)
-    if (!end.kept(z[i], at(i))) weight[i] = 0.0;
+    if (!end.kept(draw_again(z[i]), at(i))) weight[i] = 0.0;
 }
 
 // Cuts the row's top-k and top-p.  z: -inf where there is nothing; column j of z[i] from at(i); weight: of z[i].  False if
@@ -546,6 +557,68 @@ __device__ bool draw_short_narrow(const float (&z)[VPT], double (&weight)[VPT], 
     if (!draw_by_mass<THREADS, VPT>(z, weight, bins, at, 0, c.share, 0.0, shift, s, &end)) return false;
     draw_cut<VPT>(z, weight, at, end);
   }
+  return true;
+}
+
+// A row with a top-k of at most as many values as there are threads: what it leaves goes to LDS in the order of the columns,
+// one value a thread, so that weights, top-p, min-p and the draw are the work of one value a thread and not of VPT (4096
+// rows of 2000, top-k 40 and top-p: 28 us, with VPT 34).  The row's answer.  False if the border's bin holds more values
+// than there is room for.
+template <int THREADS, int VPT, typename AT>
+__device__ bool draw_short_top(const DrawArgs &a, int64_t row, const float (&z)[VPT], AT at, float max, float min, const DrawChoice &c,
+                               int shift, ShortShared<THREADS> &s)
+{
+  const DrawBin<ShortShared<THREADS>::kBins> bin(max, min, c.temp);
+  int bins[VPT];
+#pragma unroll
+  for (int i = 0; i < VPT; i++) bins[i] = bin.of(z[i]);
+  DrawEnd end{~0ull};
+  if (!draw_by_count<THREADS, VPT>(z, bins, at, (uint32_t)c.k, s, &end)) return false;
+  constexpr int kWaves = THREADS / kWave;
+  const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
+  bool keep[VPT];
+  unsigned long long kept[VPT]; // the same of all lanes
+  uint32_t n = 0;
+#pragma unroll
+  for (int i = 0; i < VPT; i++) {
+    keep[i] = z[i] > -HUGE_VALF && end.kept(draw_again(z[i]), at(i));
+    kept[i] = __ballot(keep[i]);
+    n += __popcll(kept[i]);
+  }
+  __syncthreads(); // the counts and sums of before have been read
+  if (lane == 0) s.i[wave] = n;
+  __syncthreads();
+  uint32_t before = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < kWaves; w++) {
+    const uint32_t there = s.i[w];
+    if (w < wave) before += there;
+    all += there;
+  }
+#pragma unroll
+  for (int i = 0; i < VPT; i++) {
+    const uint32_t to = __builtin_amdgcn_mbcnt_hi((uint32_t)(kept[i] >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)kept[i], before));
+    if (keep[i]) {
+      s.value[to] = z[i];
+      s.count[to] = (uint32_t)at(i);
+    }
+    before += __popcll(kept[i]);
+  }
+  __syncthreads();
+  const bool mine = (uint32_t)tid < all;
+  const float own[1] = {mine ? s.value[tid] : -HUGE_VALF};
+  const int column = mine ? (int)s.count[tid] : 0;
+  double w[1] = {draw_weight(own[0], max, c.rate)};
+  if (c.share < 1.0) {
+    const int b[1] = {bin.of(own[0])};
+    auto here = [&](int) { return column; };
+    draw_by_mass<THREADS, 1>(own, w, b, here, 0, c.share, 0.0, shift, s, &end); // (there is room for every thread's)
+    draw_cut<1>(own, w, here, end);
+  }
+  if (w[0] < c.least) w[0] = 0.0;
+  double total, weight, rest;
+  __syncthreads();
+  if (draw_pick<THREADS, 1, true>(w, c.u, &total, &weight, &rest, s.d) >= 0) draw_answer(a, row, column, log(weight / total));
   return true;
 }
 
@@ -627,12 +700,19 @@ template <typename T, int THREADS, int VPT> __global__ __launch_bounds__(THREADS
     if (tid == 0) draw_answer(a, row, s.quick.i[0], 0.0);
     return;
   }
+  const bool few = c.k && c.k <= THREADS;
+  if (few && draw_short_top<THREADS, VPT>(a, row, z, at, max, min, c, shift, s.quick)) return;
   double w[VPT];
+  auto weights = [&]() {
 #pragma unroll
-  for (int i = 0; i < VPT; i++) w[i] = draw_weight(z[i], max, c.rate);
-  if (c.k || c.share < 1.0)
-    if (!draw_short_narrow<THREADS, VPT>(z, w, at, max, min, c, shift, s.quick))
-      draw_cut<VPT>(z, w, at, draw_whole<T, THREADS>(a, row, c, max, shift, s.whole)); // (after a cut by top-k the same end, or an earlier one)
+    for (int i = 0; i < VPT; i++) w[i] = draw_weight(draw_again(z[i]), max, c.rate);
+  };
+  if (!few) weights();
+  if (few || ((c.k || c.share < 1.0) && !draw_short_narrow<THREADS, VPT>(z, w, at, max, min, c, shift, s.quick))) {
+    const DrawEnd end = draw_whole<T, THREADS>(a, row, c, max, shift, s.whole);
+    weights(); // again, so that they take no registers in there
+    draw_cut<VPT>(z, w, at, end);
+  }
 #pragma unroll
   for (int i = 0; i < VPT; i++)
     if (w[i] < c.least) w[i] = 0.0;
