@@ -271,8 +271,8 @@ template <typename T> int draw_part(const DrawArgs &a, const DrawPlan &p, int sh
 {
   if (p.short_rows) {
     // Many rows: few waves a row, since a wave's own cost (scans, the border) adds up (top-k, top-p and min-p, 4096 rows:
-    // of 2000, 4 waves 39 us, 8 waves 47; of 400, 1 wave 14 us, 4 waves 20).  Few rows: as many waves as there is work
-    // for, which shortens a row's chain of steps (1 row of 1000: 8 waves 7.1 us, 4 waves 8.4).
+    // of 2000, 4 waves 28 us, 8 waves 41; of 400, 1 wave 11 us, 4 waves 20; 512 rows are about even).  Few rows: as many
+    // waves as there is work for, which shortens a row's chain of steps (1 row of 1000: 8 waves 7.1 us, 4 waves 8.4).
     const dim3 grid((unsigned)a.rows);
     const bool many = a.rows >= 512;
     if (many && a.n <= 128)
