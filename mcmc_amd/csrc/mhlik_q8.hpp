@@ -97,16 +97,6 @@ template <typename T> __device__ __forceinline__ void q8_eight(const Q8Values &x
   }
 }
 
-__device__ __forceinline__ void q8_eight(const Q8Values &x, int64_t row, int64_t c0, int64_t n, float (&v)[kQ8Lane])
-{
-  switch (x.type) {
-  case 1: return q8_eight<double>(x, row, c0, n, v);
-  case 2: return q8_eight<float>(x, row, c0, n, v);
-  case 3: return q8_eight<__bf16>(x, row, c0, n, v);
-  default: return q8_eight<_Float16>(x, row, c0, n, v);
-  }
-}
-
 // A block's share of one of 16 lanes: its eight values as bytes, and k.
 __device__ __forceinline__ uint2 q8_pack_block(const float (&v)[kQ8Lane], int *k)
 {
@@ -257,6 +247,33 @@ struct Q8Product {
   int64_t os;                     // row stride of C
 };
 
+// A workgroup's units (blocks of rows, row by row) to bytes and scales in LDS, 16 lanes a unit, the loads of a few of them
+// under way together.
+template <typename T>
+__device__ __forceinline__ void q8_pack_units(const Q8Values &x, int units, int blocks, int64_t cols, uint8_t *bytes, uint8_t *codes)
+{
+  constexpr int kAtOnce = 4;
+  const int l = threadIdx.x & 15, step = blockDim.x / 16;
+#pragma unroll 1
+  for (int u0 = threadIdx.x / 16; u0 < units; u0 += step * kAtOnce) {
+    float v[kAtOnce][kQ8Lane];
+#pragma unroll
+    for (int q = 0; q < kAtOnce; q++) {
+      const int unit = u0 + q * step, row = unit / blocks;
+      if (unit < units) q8_eight<T>(x, row, (int64_t)(unit - row * blocks) * kQ8Block + l * kQ8Lane, cols, v[q]);
+    }
+#pragma unroll
+    for (int q = 0; q < kAtOnce; q++) {
+      const int unit = u0 + q * step;
+      if (unit < units) { // whole groups of 16 lanes
+        int k;
+        *(uint2 *)(bytes + unit * kQ8Block + l * kQ8Lane) = q8_pack_block(v[q], &k);
+        if (l == 0) codes[unit] = (uint8_t)(k + 127);
+      }
+    }
+  }
+}
+
 // Few rows (up to 16 a fragment, RF fragments): what bounds it is reading the draws once.  A wave takes 16 draws and every
 // ks-th block of 128 columns; its lanes load a draw's bytes straight into the instruction's operand, 4 lanes a block, four
 // blocks ahead, each into the registers of the one just taken up (1 row x 8192 draws x 8192 in 8 bits: 17.4 us, 3.9 TB/s;
@@ -289,15 +306,12 @@ __global__ __launch_bounds__(512) void q8_skinny_kernel(Q8Product a, Q8Values va
     if (kw + q * ks < a.blocks) fetch(q, kw + q * ks);
   uint8_t *bytes = (uint8_t *)part;
   if (FROM_VALUES) {
-    const int l = tid & 15, units = (int)a.rows * a.blocks;
-    for (int unit = tid / 16; unit < units; unit += blockDim.x / 16) {
-      const int row = unit / a.blocks;
-      const int64_t c0 = (int64_t)(unit - row * a.blocks) * kQ8Block + l * kQ8Lane;
-      float v[kQ8Lane];
-      q8_eight(values, row, c0, a.cols, v);
-      int k;
-      *(uint2 *)(bytes + unit * kQ8Block + l * kQ8Lane) = q8_pack_block(v, &k);
-      if (l == 0) codes[unit] = (uint8_t)(k + 127);
+    const int units = (int)a.rows * a.blocks;
+    switch (values.type) {
+    case 1: q8_pack_units<double>(values, units, a.blocks, a.cols, bytes, codes); break;
+    case 2: q8_pack_units<float>(values, units, a.blocks, a.cols, bytes, codes); break;
+    case 3: q8_pack_units<__bf16>(values, units, a.blocks, a.cols, bytes, codes); break;
+    default: q8_pack_units<_Float16>(values, units, a.blocks, a.cols, bytes, codes); break;
     }
     __syncthreads();
   }
