@@ -354,7 +354,7 @@ __device__ void draw_narrow(DrawRow<T> &r, DrawShared &s, int shift, uint32_t k,
   } else {
     take = k - above_n;
   }
-  int last = r.n;
+  int last = prefix == r.key ? r.last : r.n; // a border among the same values stands: none of those behind it comes back
   if (take < equal) { // find the column: waves count in runs of columns, then one wave looks through the right run
     constexpr int kWaves = THREADS / kWave;
     const int run = ((r.n + kWaves - 1) / kWaves + kWave - 1) / kWave * kWave;

@@ -631,3 +631,18 @@ def test_threads_at_once(P):
     for t in threads:
         t.join()
     assert not wrong
+
+
+@pytest.mark.parametrize("rows,n", [(515, 100), (515, 400), (3, 400), (515, 1500), (515, 3000), (3, 5000), (3, 30000), (1, (1 << 21) + 5)])
+def test_draw_both_borders_among_the_same_ties(P, rows, n):
+    """top-k cuts a run of equal weights, and top-p needs all of what is left of it: the run's other columns stay out."""
+    g = torch.Generator(device="cuda").manual_seed(rows + n)
+    u = torch.rand(rows, generator=g, device="cuda", dtype=torch.float64)
+    flat = torch.full((rows, n), -1.25, device="cuda")
+    two = torch.where(torch.rand(rows, n, generator=g, device="cuda") < 0.2, 0.0, flat)  # the border lies in the lower, larger run
+    for z in (flat, two, two.bfloat16()):
+        for choice in (dict(top_k=10, top_p=0.95), dict(top_k=n // 2, top_p=0.99999), dict(top_k=n - 1, top_p=0.9999, min_p=0.1)):
+            check_draw(P, z, u, **choice)
+    k = torch.randint(1, n, (rows,), generator=g, device="cuda", dtype=torch.int32)
+    p = 1.0 - 1e-5 * torch.rand(rows, generator=g, device="cuda")
+    check_draw(P, two, u, 0.7, k, p)
