@@ -489,7 +489,8 @@ int mhlik_q8_product(const mhlik_q8_operands *operands, int32_t device, void *st
  *     those with w_j >= min(min_p, 1)                              (min_p <= 0: all)
  *   index[i] = the first column, in column order, at which the kept mass exceeds u of the whole of it
  *   logp[i]  = log(w_index / kept mass)                            (logp may be NULL)
- * Sums are taken in double.  temperature 0: the largest, the lowest column of equal ones.  A row without a weight above
+ * Sums are taken in double; those that decide where top_p ends, in whole multiples of 2^-51 of the largest weight (of more
+ * where the sum needs the bits: n 2^-51 of the mass off at most).  temperature 0: the largest, the lowest column of equal ones.  A row without a weight above
  * -inf, with a NaN, or whose u, temperature, top_p or min_p is NaN (or the temperature negative): index -1, logp NaN.
  * u outside [0, 1) counts as its nearest end.  temperature .. min_p: device arrays of one value a row, or NULL and the
  * *_all value for every row.  0 <= rows < 2^31, 1 <= n < 2^30. */

@@ -14,8 +14,8 @@
 //
 // u is compared with sums of up to n weights, so weights and sums are double: with float sums a draw among 1e5 weights
 // would land in a neighbouring column once in a few hundred draws.  Sums that pick a border are taken in 64-bit whole
-// numbers (weights to 2^-51, or 2^-63 n if that is more), so that the order of atomic additions does not matter; the
-// sums u is compared with have a fixed shape.
+// numbers (weights to 2^-51, or 2^-62 of what bounds their sum if that is more: n 2^-51 of the mass at most in all), so that
+// the order of atomic additions does not matter; the sums u is compared with have a fixed shape.
 #pragma once
 
 #include "mhlik_predict.hpp"
@@ -144,6 +144,20 @@ __device__ __forceinline__ unsigned long long draw_fixed(double w, int shift)
   const int one = (1023 + 52 - shift) << 20;
   const double v = w + __hiloint2double(one, 0);
   return (unsigned long long)(uint32_t)(__double2hiint(v) - one) << 32 | (uint32_t)__double2loint(v);
+}
+
+// A weight to within 2e-5 relative (or 2^-126), for bounds: float's own instruction.
+__device__ __forceinline__ float draw_rough(float z, float max, double rate)
+{
+  const float y = fmaxf((z - max) * (float)fmin(rate, 0x1p127), -126.f); // NaN (-inf * 0) too
+  return __builtin_amdgcn_exp2f(y);
+}
+
+// The finest shift, up to 51, at which sums of up to `bound` (at least 1) stay below 2^63.
+__device__ __forceinline__ int draw_shift(float bound)
+{
+  const int e = (int)(__float_as_uint(bound) >> 23) - 127; // bound < 2^(e + 1)
+  return __builtin_amdgcn_readfirstlane(e > 11 ? 62 - e : 51); // all lanes have the same
 }
 
 // Position in the order: smaller is earlier (larger value, lower column).
@@ -755,6 +769,7 @@ struct LongCell { // one row's border bin
   int too_long;
   unsigned long long above;
   double target;
+  int shift;
 };
 
 struct LongCand {
@@ -769,6 +784,7 @@ struct LongSpace {
   LongCand *list;           // [rows][units][unit / 2]
   unsigned long long *histo; // [rows][kLongBins]
   LongCell *cell;           // [rows]
+  int *shift;               // [rows]
   int units, groups;        // per row: waves, workgroups of four
 };
 
@@ -784,8 +800,8 @@ __device__ inline int draw_kind(const DrawChoice &c, bool bad, float max)
   return __builtin_amdgcn_readfirstlane(kind); // all lanes have the same
 }
 
-// The row's largest and smallest value from its units'; every wave does it for itself.
-__device__ inline void draw_row_range(const LongPart *part, int units, float *max, float *min, bool *nan)
+// The row's largest and smallest value from its units'; every wave does it for itself.  *own: the largest of this lane's units.
+__device__ inline void draw_row_range(const LongPart *part, int units, float *max, float *min, bool *nan, float *own)
 {
   float a = -HUGE_VALF, b = HUGE_VALF;
   int bad = 0;
@@ -794,9 +810,23 @@ __device__ inline void draw_row_range(const LongPart *part, int units, float *ma
     b = fminf(b, part[q].min);
     bad |= part[q].nan;
   }
+  *own = a;
   *max = wave_max(a);
   *min = wave_min(b);
   *nan = __any(bad) != 0;
+}
+
+// The shift of a row's masses, from what its units can weigh at most: n alone as the bound would lose weights that are
+// faint but many (of 2^21 columns, 2^-44 each beside one of 1: 2^-23 of the mass, and none would count).  The units'
+// largest values weigh a unit-th of the bound at least, so that all roundings together stay below n 2^-51 of the mass.
+__device__ inline int draw_row_shift(const LongPart *part, int units, int unit, float max, float own, double rate)
+{
+  float b = draw_rough(own, max, rate);
+  if (units > kWave) { // a lane has several
+    b = 0.f;
+    for (int q = threadIdx.x % kWave; q < units; q += kWave) b += draw_rough(part[q].max, max, rate);
+  }
+  return draw_shift(1.001f * unit * wave_sum(b));
 }
 
 // A unit's values: register v * VEC + e of lane l holds column base + (v * 64 + l) * VEC + e; -inf past the end.  True if
@@ -876,7 +906,7 @@ __global__ __launch_bounds__(kBlock) void draw_top_kernel(DrawArgs a, LongSpace 
 constexpr int kAtOnce = 8;
 
 template <typename T, int VEC, int VPT>
-__global__ __launch_bounds__(kBlock) void draw_histo_kernel(DrawArgs a, LongSpace g, int groups, int shift)
+__global__ __launch_bounds__(kBlock) void draw_histo_kernel(DrawArgs a, LongSpace g, int groups)
 {
   __shared__ unsigned long long bins[kLongBins];
   const int64_t row = blockIdx.x / groups;
@@ -885,15 +915,17 @@ __global__ __launch_bounds__(kBlock) void draw_histo_kernel(DrawArgs a, LongSpac
   int unit = group * 4 + wave;
   float z[VPT]; // on their way before it is known what the row needs
   if (unit < g.units) draw_load<T, VEC, VPT>(zp, (int)a.n, unit * VPT * kWave, z);
-  float max, min;
+  float max, min, own;
   bool nan;
-  draw_row_range(g.part + row * g.units, g.units, &max, &min, &nan);
+  draw_row_range(g.part + row * g.units, g.units, &max, &min, &nan, &own);
   const DrawChoice c = draw_choice(a, row);
   const int kind = draw_kind(c, nan, max);
   if (kind != kRowList && kind != kRowNucleus) return;
   for (int b = threadIdx.x; b < kLongBins; b += kBlock) bins[b] = 0;
   __syncthreads();
   const DrawBin<kLongBins> bin(max, min, c.temp);
+  const int shift = kind == kRowNucleus ? draw_row_shift(g.part + row * g.units, g.units, VPT * kWave, max, own, c.rate) : 0;
+  if (kind == kRowNucleus && group == 0 && threadIdx.x == 0) g.shift[row] = shift;
   while (unit < g.units) {
     if (kind == kRowList) {
 #pragma unroll
@@ -919,7 +951,7 @@ __global__ __launch_bounds__(kBlock) void draw_histo_kernel(DrawArgs a, LongSpac
 }
 
 template <typename T, int VEC, int VPT>
-__global__ __launch_bounds__(kBlock) void draw_collect_kernel(DrawArgs a, LongSpace g, int shift)
+__global__ __launch_bounds__(kBlock) void draw_collect_kernel(DrawArgs a, LongSpace g)
 {
   __shared__ unsigned long long sums[kBlock / kWave];
   __shared__ LongCell cell;
@@ -929,9 +961,10 @@ __global__ __launch_bounds__(kBlock) void draw_collect_kernel(DrawArgs a, LongSp
   const int u = group * 4 + wave;
   float z[VPT];
   if (u < g.units) draw_load<T, VEC, VPT>((const T *)a.z + row * a.stride, (int)a.n, u * kUnit, z);
-  float max, min;
+  const int shift = g.shift[row]; // of rows with a nucleus
+  float max, min, own;
   bool nan;
-  draw_row_range(g.part + row * g.units, g.units, &max, &min, &nan);
+  draw_row_range(g.part + row * g.units, g.units, &max, &min, &nan, &own);
   const DrawChoice c = draw_choice(a, row);
   const int kind = draw_kind(c, nan, max);
   if (kind < kRowSums) return;
@@ -947,7 +980,7 @@ __global__ __launch_bounds__(kBlock) void draw_collect_kernel(DrawArgs a, LongSp
     }
     unsigned long long in = wave_running(mine);
     if (lane == kWave - 1) sums[wave] = in;
-    if (tid == 0) cell = LongCell{kLongBins - 1, 0, 0, 0.0};
+    if (tid == 0) cell = LongCell{kLongBins - 1, 0, 0, 0.0, shift};
     __syncthreads();
     unsigned long long all = 0;
 #pragma unroll
@@ -962,7 +995,7 @@ __global__ __launch_bounds__(kBlock) void draw_collect_kernel(DrawArgs a, LongSp
       const unsigned long long after = before + h[i];
       const bool here = kind == kRowList ? before < (unsigned long long)c.k && after >= (unsigned long long)c.k
                                          : h[i] && ((double)before * unit < target || before == 0) && (double)after * unit >= target;
-      if (here) cell = LongCell{tid * kRun + i, kind == kRowList && after > kLongList, before, target};
+      if (here) cell = LongCell{tid * kRun + i, kind == kRowList && after > kLongList, before, target, shift};
       before = after;
     }
     if (kind == kRowList && tid == 0 && all < (unsigned long long)c.k) cell.too_long = all > kLongList; // fewer values than k: all
@@ -1015,7 +1048,7 @@ __global__ __launch_bounds__(kBlock) void draw_collect_kernel(DrawArgs a, LongSp
 }
 
 // One workgroup of 1024 a row.
-template <typename T, int VPT> __global__ __launch_bounds__(1024) void draw_finish_kernel(DrawArgs a, LongSpace g, int shift)
+template <typename T, int VPT> __global__ __launch_bounds__(1024) void draw_finish_kernel(DrawArgs a, LongSpace g)
 {
   constexpr int kThreads = 1024, kUnit = VPT * kWave, kIn = (kUnit + kThreads - 1) / kThreads;
   __shared__ RowShared<kThreads> s;
@@ -1026,9 +1059,9 @@ template <typename T, int VPT> __global__ __launch_bounds__(1024) void draw_fini
   const int64_t row = blockIdx.x;
   const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
   const LongPart *part = g.part + row * g.units;
-  float max, min;
+  float max, min, own;
   bool nan;
-  draw_row_range(part, g.units, &max, &min, &nan);
+  draw_row_range(part, g.units, &max, &min, &nan, &own);
   const DrawChoice c = draw_choice(a, row);
   const int kind = draw_kind(c, nan, max);
   if (kind == kRowNothing) {
@@ -1048,9 +1081,11 @@ template <typename T, int VPT> __global__ __launch_bounds__(1024) void draw_fini
   DrawEnd end{~0ull};
   bool whole = false;
   int listed = 0;
-  LongCell cell{0, 0, 0, 0.0};
+  LongCell cell{0, 0, 0, 0.0, 0};
+  int shift = 51; // at which kLongList of them stay below 2^63
   if (kind >= kRowList) {
     cell = g.cell[row];
+    if (kind == kRowNucleus) shift = __builtin_amdgcn_readfirstlane(cell.shift);
     whole = cell.too_long != 0;
     int mine = 0, in = 0;
     if (!whole) {
@@ -1130,7 +1165,10 @@ template <typename T, int VPT> __global__ __launch_bounds__(1024) void draw_fini
   }
   const T *zp = (const T *)a.z + row * a.stride;
   const int n = (int)a.n;
-  if (whole) end = draw_whole<T, kThreads>(a, row, c, max, shift, s.whole);
+  if (whole) {
+    shift = draw_row_shift(part, g.units, kUnit, max, own, c.rate);
+    end = draw_whole<T, kThreads>(a, row, c, max, shift, s.whole);
+  }
   // The kept mass of each unit
   auto weight_of = [&](float z, int j) {
     const double w = z > -HUGE_VALF && end.kept(z, j) ? draw_weight(z, max, c.rate) : 0.0;
@@ -1182,7 +1220,7 @@ template <typename T, int VPT> __global__ __launch_bounds__(1024) void draw_fini
 }
 
 // Rows too long for the units: one workgroup a row, whole-row ways only.
-template <typename T> __global__ __launch_bounds__(1024) void draw_huge_kernel(DrawArgs a, int shift)
+template <typename T> __global__ __launch_bounds__(1024) void draw_huge_kernel(DrawArgs a)
 {
   constexpr int kThreads = 1024, kWaves = kThreads / kWave;
   __shared__ DrawShared s;
@@ -1191,14 +1229,18 @@ template <typename T> __global__ __launch_bounds__(1024) void draw_huge_kernel(D
   const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave, n = (int)a.n;
   const T *zp = (const T *)a.z + row * a.stride;
   const DrawChoice c = draw_choice(a, row);
-  float max = -HUGE_VALF;
+  float own = -HUGE_VALF, mass = 0.f; // the mass, relative to the largest so far: of up to 2^20 values, a sixteenth too small at worst
   bool nan = false;
   for (int j = tid; j < n; j += kThreads) {
-    const float z = (float)zp[j];
-    nan |= z != z;
-    max = fmaxf(max, draw_finite(z));
+    const float v = (float)zp[j], z = draw_finite(v);
+    nan |= v != v;
+    if (z > own) {
+      mass *= draw_rough(own, z, c.rate);
+      own = z;
+    }
+    mass += draw_rough(z, own, c.rate);
   }
-  max = wave_max(max);
+  float max = wave_max(own);
   const bool any = __any(nan);
   if (lane == 0) {
     s.f[wave] = max;
@@ -1212,6 +1254,12 @@ template <typename T> __global__ __launch_bounds__(1024) void draw_huge_kernel(D
     bad |= s.i[w] != 0;
   }
   __syncthreads();
+  mass = wave_sum(mass * draw_rough(own, max, c.rate));
+  if (lane == 0) s.f[wave] = mass;
+  __syncthreads();
+  mass = 0.f;
+  for (int w = 0; w < kWaves; w++) mass += s.f[w];
+  const int shift = draw_shift(1.1f * mass);
   if (bad || max == -HUGE_VALF) {
     if (tid == 0) draw_nothing(a, row);
     return;

@@ -250,26 +250,28 @@ DrawPlan draw_plan(int64_t rows, int64_t n, void *workspace)
   g.listed = (int *)take(sizeof(int) * rows * units);
   g.histo = (unsigned long long *)take(sizeof(unsigned long long) * rows * kLongBins);
   g.cell = (LongCell *)take(sizeof(LongCell) * rows);
+  g.shift = (int *)take(sizeof(int) * rows);
   g.list = (LongCand *)take(sizeof(LongCand) * rows * units * (unit / 2));
   return p;
 }
 
-template <typename T, int VEC, int VPT> void draw_long(const DrawArgs &a, const LongSpace &g, int shift, bool histo, bool collect, hipStream_t stream)
+template <typename T, int VEC, int VPT> void draw_long(const DrawArgs &a, const LongSpace &g, bool histo, bool collect, hipStream_t stream)
 {
   const dim3 grid((unsigned)(a.rows * g.groups));
   hipLaunchKernelGGL((draw_top_kernel<T, VEC, VPT>), grid, dim3(kBlock), 0, stream, a, g, (int)histo);
   if (histo) { // a workgroup's histogram is added to the row's at the end: no more workgroups than fill the chip four times
     int groups = g.groups;
     while (groups > 1 && a.rows * groups > 1024) groups = (groups + 1) / 2;
-    hipLaunchKernelGGL((draw_histo_kernel<T, VEC, VPT>), dim3((unsigned)(a.rows * groups)), dim3(kBlock), 0, stream, a, g, groups, shift);
+    hipLaunchKernelGGL((draw_histo_kernel<T, VEC, VPT>), dim3((unsigned)(a.rows * groups)), dim3(kBlock), 0, stream, a, g, groups);
   }
-  if (collect) hipLaunchKernelGGL((draw_collect_kernel<T, VEC, VPT>), grid, dim3(kBlock), 0, stream, a, g, shift);
-  hipLaunchKernelGGL((draw_finish_kernel<T, VPT>), dim3((unsigned)a.rows), dim3(1024), 0, stream, a, g, shift);
+  if (collect) hipLaunchKernelGGL((draw_collect_kernel<T, VEC, VPT>), grid, dim3(kBlock), 0, stream, a, g);
+  hipLaunchKernelGGL((draw_finish_kernel<T, VPT>), dim3((unsigned)a.rows), dim3(1024), 0, stream, a, g);
 }
 
-template <typename T> int draw_part(const DrawArgs &a, const DrawPlan &p, int shift, hipStream_t stream)
+template <typename T> int draw_part(const DrawArgs &a, const DrawPlan &p, hipStream_t stream)
 {
   if (p.short_rows) {
+    const int shift = a.n <= 4096 ? 51 : 50; // weights in whole numbers: n of them, of 1 at most, stay below 2^63
     // Many rows: few waves a row, since a wave's own cost (scans, the border) adds up (top-k, top-p and min-p, 4096 rows:
     // of 2000, 4 waves 28 us, 8 waves 41; of 400, 1 wave 11 us, 4 waves 20; 512 rows are about even).  Few rows: as many
     // waves as there is work for, which shortens a row's chain of steps (1 row of 1000: 8 waves 7.1 us, 4 waves 8.4).
@@ -290,15 +292,15 @@ template <typename T> int draw_part(const DrawArgs &a, const DrawPlan &p, int sh
     else
       hipLaunchKernelGGL((draw_short_kernel<T, 1024, 8>), grid, dim3(1024), 0, stream, a, shift);
   } else if (!p.vpt) {
-    hipLaunchKernelGGL(draw_huge_kernel<T>, dim3((unsigned)a.rows), dim3(1024), 0, stream, a, shift);
+    hipLaunchKernelGGL(draw_huge_kernel<T>, dim3((unsigned)a.rows), dim3(1024), 0, stream, a);
   } else {
     const bool histo = a.top_k || a.top_p || (a.top_k_all > 0 && a.top_k_all < a.n) || a.top_p_all < 1.0;
     const bool collect = histo || a.min_p || a.min_p_all > 0.0;
     constexpr int kVec = 16 / sizeof(T);
     if (p.vpt == 16)
-      draw_long<T, kVec, 16>(a, p.space, shift, histo, collect, stream);
+      draw_long<T, kVec, 16>(a, p.space, histo, collect, stream);
     else
-      draw_long<T, kVec, kLongVpt>(a, p.space, shift, histo, collect, stream);
+      draw_long<T, kVec, kLongVpt>(a, p.space, histo, collect, stream);
   }
   PCHK(hipGetLastError());
   return MHLIK_OK;
@@ -306,11 +308,9 @@ template <typename T> int draw_part(const DrawArgs &a, const DrawPlan &p, int sh
 
 template <typename T> int draw_launch(DrawArgs a, const DrawPlan &p, hipStream_t stream)
 {
-  int shift = 51; // weights in whole numbers: n of them stay below 2^63
-  while (((int64_t)1 << (63 - shift)) < a.n) shift--;
   for (int64_t left = a.rows; left > 0; left -= p.part) {
     const int64_t rows = a.rows = std::min(left, p.part);
-    if (int rc = draw_part<T>(a, p, shift, stream)) return rc;
+    if (int rc = draw_part<T>(a, p, stream)) return rc;
     a.z = (const T *)a.z + rows * a.stride;
     a.u = (const char *)a.u + rows * (a.u_is_double ? 8 : 4);
     if (a.temperature) a.temperature += rows;

@@ -646,3 +646,43 @@ def test_draw_both_borders_among_the_same_ties(P, rows, n):
     k = torch.randint(1, n, (rows,), generator=g, device="cuda", dtype=torch.int32)
     p = 1.0 - 1e-5 * torch.rand(rows, generator=g, device="cuda")
     check_draw(P, two, u, 0.7, k, p)
+
+
+@pytest.mark.parametrize("n,spread", [(150_000, 3.9), (1 << 21, 0.0), (1 << 24, 0.0)], ids=["listed", "long", "huge"])
+def test_draw_nucleus_of_faint_weights(P, n, spread):
+    """One weight of 1, and behind it so many faint ones that they have a mass, of which top-p keeps half.  The border is
+    found with weights to 2^-51, 2^-52 off each at most, and sums in double: a draw is off by n 2^-51 of the mass at most."""
+    g = torch.Generator(device="cuda").manual_seed(n)
+    z = -36.0 + spread * (2 * torch.rand(1, n, generator=g, device="cuda") - 1)
+    z[0, n - 1] = 0.0
+    w = np.exp(z[0].double().cpu().numpy()).astype(np.longdouble)
+    tail = w[:-1].sum()
+    top_p = float(1 - tail / 2 / (1 + tail))
+    order = np.lexsort((np.arange(n), -w))
+    mass = np.cumsum(w[order])
+    kept = order[: int(np.searchsorted(mass, top_p * mass[-1])) + 1]
+    weight = np.zeros(n, np.longdouble)
+    weight[kept] = w[kept]
+    upto = np.cumsum(weight)
+    for share in (0.1, 0.25, 0.4):
+        u = float(share * tail)
+        column, logp = P.draw(z, torch.tensor([u], dtype=torch.float64, device="cuda"), top_p=top_p)
+        column = int(column)
+        assert column < n - 1 and weight[column] > 0
+        aim, off = u * upto[-1], n * 2.0 ** -51
+        assert upto[column] - weight[column] - off <= aim <= upto[column] + off
+        assert abs(float(logp) - math.log(weight[column])) <= 2.0 ** -24 * 40 + n * 2.0 ** -51
+
+
+def test_draw_masks_in_rows_too_long_for_units(P):
+    """A NaN, nothing but -inf, +inf, the type's lowest value: the way of one workgroup a row."""
+    n = (1 << 21) + 7
+    g = torch.Generator(device="cuda").manual_seed(n)
+    z = random_row(g, 5, n, torch.bfloat16)
+    z[0, n - 2] = math.nan
+    z[1] = -math.inf
+    z[2, n // 3] = math.inf
+    z[3] = torch.where(torch.rand(n, generator=g, device="cuda") < 0.999, torch.finfo(torch.bfloat16).min, z[3])
+    u = torch.rand(5, generator=g, device="cuda", dtype=torch.float64)
+    for choice in (dict(), dict(temperature=0.0), dict(top_p=0.8), dict(temperature=0.5, top_k=50, top_p=0.9, min_p=0.001)):
+        check_draw(P, z, u, **choice)
