@@ -44,6 +44,11 @@ def _given(name, t, dims, types):
     raise ValueError("%s requires a gradient, and there is none: detach it" % name)
 
 
+def _plain(t):
+    """t, whose memory holds its values as they are: torch keeps the sign of, for one, c.conj().imag as a mark only."""
+    return t.resolve_neg() if t.is_neg() else t
+
+
 def _same(name, device, wanted):
     if device != wanted:
         raise ValueError("%s is on %s, the rest on %s" % (name, device, wanted))
@@ -87,6 +92,7 @@ def quantize(x):
     device = _given("x", x, 2, _TYPES)
     rows, cols = x.shape
     _need(cols >= 1, "x must have at least one column")
+    x = _plain(x)
     blocks = -(-cols // BLOCK)
     q = Block8.__new__(Block8)  # as its constructor would have it
     q.data = torch.empty((rows, blocks * BLOCK), dtype=torch.float8_e4m3fn, device=device)
@@ -121,6 +127,7 @@ def product(x, w, dtype=torch.float32):
     else:
         _same("x", _given("x", x, 2, _TYPES), device)
         rows, cols = x.shape
+        x = _plain(x)
         p.x, p.x_type = x.data_ptr(), _TYPES[x.dtype]
         p.x_row_stride, p.x_col_stride = x.stride()
     if cols != w.cols:
@@ -144,7 +151,7 @@ def _each(name, value, kind, rows, device):
     """A choice that every row has its own of."""
     _same(name, _given(name, value, 1, kind), device)
     _need(value.shape[0] == rows, "%s has %d values for %d rows", name, value.shape[0], rows)
-    return value.contiguous()
+    return _plain(value).contiguous()
 
 
 _F32, _I32 = {torch.float32: None}, {torch.int32: None}
@@ -171,6 +178,7 @@ def draw(z, u, temperature=1.0, top_k=None, top_p=None, min_p=None):
     rows, n = z.shape
     _need(n >= 1, "z must have at least one column")
     _need(u.shape[0] == rows, "u has %d values for %d rows", u.shape[0], rows)
+    z, u = _plain(z), _plain(u)
     stride, step = z.stride()
     if step != 1 and n > 1:
         z = z.contiguous()

@@ -686,3 +686,32 @@ def test_draw_masks_in_rows_too_long_for_units(P):
     u = torch.rand(5, generator=g, device="cuda", dtype=torch.float64)
     for choice in (dict(), dict(temperature=0.0), dict(top_p=0.8), dict(temperature=0.5, top_k=50, top_p=0.9, min_p=0.001)):
         check_draw(P, z, u, **choice)
+
+
+def test_tensors_with_the_negative_bit(P):
+    """torch keeps the sign of c.conj().imag as a mark on the tensor; the memory holds the other sign."""
+    g = torch.Generator(device="cuda").manual_seed(4)
+
+    def negative(v):
+        t = torch.complex(torch.zeros_like(v), -v).conj().imag
+        assert t.is_neg() and torch.equal(t, v)
+        return t
+
+    x, z = torch.randn(3, 200, generator=g, device="cuda"), torch.randn(3, 70, generator=g, device="cuda")
+    w = P.quantize(torch.randn(40, 200, generator=g, device="cuda"))
+    check_quantized(P, negative(x))
+    check_quantized(P, negative(x.double()))
+    assert torch.equal(P.product(negative(x), w), P.product(x, w))
+    many = torch.randn(100, 200, generator=g, device="cuda")
+    assert torch.equal(P.product(negative(many), w), P.product(many, w))
+    u = torch.rand(3, generator=g, device="cuda")
+    each = [torch.tensor(v, device="cuda") for v in ([0.5, 1.0, 2.0], [0.9, 0.8, 0.5], [0.01, 0.1, 0.2])]
+    for rows in (3, 1):  # one value a row: contiguous at any stride
+        t, p, m = (negative(v[:rows]) for v in each)
+        want = P.draw(z[:rows], u[:rows], each[0][:rows], 30, each[1][:rows], each[2][:rows])
+        got = P.draw(negative(z[:rows]), negative(u[:rows]), t, 30, p, m)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    empty = negative(torch.full((2, 1), -math.inf, device="cuda"))
+    assert P.draw(empty, u[:2])[0].tolist() == [-1, -1]
+    pp = P.PosteriorPredictive(negative(x))
+    assert torch.equal(pp.probability(negative(many)), P.PosteriorPredictive(x).probability(many))
