@@ -3,12 +3,14 @@
 `quantize` holds rows in 8 bits, `product` gives the predictor x_i.theta_s of every row under every draw, `draw` picks a
 column of each row of log weights by a given random number; `PosteriorPredictive` is the three together for the draws a
 sampler has kept.  Work is queued on the tensors' GPU, on torch's current stream there; nothing waits for it.  None of
-it has gradients: inputs that require them are refused while gradients are recorded.
+it has gradients: inputs that require them are refused while gradients are recorded, and so are forward-mode tensors with
+a tangent.
 """
 import ctypes as C
 import functools
 
 import torch
+import torch.autograd.forward_ad as forward_ad
 
 from . import _lib as L
 
@@ -33,14 +35,20 @@ def _need(ok, text, *args):
         raise ValueError(text % args if args else text)
 
 
+def _dual(t):
+    return forward_ad.unpack_dual(t).tangent is not None
+
+
 def _given(name, t, dims, types):
     """The tensor's device, after the checks that every argument has to pass."""
-    if isinstance(t, torch.Tensor) and t.is_cuda and t.dim() == dims and t.dtype in types and not (t.requires_grad and _grad()):
+    if (isinstance(t, torch.Tensor) and t.is_cuda and t.dim() == dims and t.dtype in types and not (t.requires_grad and _grad())
+            and (getattr(forward_ad, "_current_level", 0) < 0 or not _dual(t))):  # outside forward_ad.dual_level there are no tangents
         return t.device
     _need(isinstance(t, torch.Tensor), "%s must be a tensor", name)
     _need(t.is_cuda, "%s must be on a GPU: there is no CPU path", name)
     _need(t.dim() == dims, "%s must have %d dimension(s), not %d", name, dims, t.dim())
     _need(t.dtype in types, "%s has type %s; wanted: %s", name, t.dtype, ", ".join(str(x) for x in types))
+    _need(not _dual(t), "%s has a tangent, and there is no gradient: detach it", name)
     raise ValueError("%s requires a gradient, and there is none: detach it" % name)
 
 

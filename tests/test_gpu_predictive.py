@@ -715,3 +715,24 @@ def test_tensors_with_the_negative_bit(P):
     assert P.draw(empty, u[:2])[0].tolist() == [-1, -1]
     pp = P.PosteriorPredictive(negative(x))
     assert torch.equal(pp.probability(negative(many)), P.PosteriorPredictive(x).probability(many))
+
+
+def test_forward_mode_is_refused(P):
+    """A dual tensor's tangent would be lost."""
+    import torch.autograd.forward_ad as forward
+
+    x, w = torch.randn(3, 200, device="cuda"), P.quantize(torch.randn(5, 200, device="cuda"))
+    z, u = torch.randn(3, 70, device="cuda"), torch.rand(3, device="cuda")
+    pp = P.PosteriorPredictive(torch.randn(6, 200, device="cuda"))
+    with forward.dual_level():
+        def dual(t):
+            return forward.make_dual(t, torch.ones_like(t))
+
+        for call in (lambda: P.quantize(dual(x)), lambda: P.product(dual(x), w), lambda: P.draw(dual(z), u), lambda: P.draw(z, dual(u)), lambda: P.draw(z, u, dual(u)),
+                     lambda: pp.probability(dual(x)), lambda: pp.case_deletion(dual(x), u)):
+            with pytest.raises(ValueError, match="tangent"):
+                call()
+        plain = P.product(x, w), P.draw(z, u)  # tensors without a tangent
+        assert torch.equal(P.product(dual(x).detach(), w), plain[0])
+        assert torch.equal(P.PosteriorPredictive(dual(x)).theta.scale, P.quantize(x).scale)  # keeps its draws detached
+    assert torch.equal(P.product(x, w), plain[0]) and torch.equal(P.draw(z, u)[0], plain[1][0])
