@@ -15,13 +15,28 @@ using namespace mhlik;
 
 namespace {
 
-#define PCHK(expr)                                                                                             \
-  do {                                                                                                         \
-    hipError_t e_ = (expr);                                                                                    \
-    if (e_ != hipSuccess)                                                                                      \
-      return fail_no_ctx(e_ == hipErrorOutOfMemory ? MHLIK_ENOMEM : MHLIK_EHIP, "%s failed: %s (%s:%d)", #expr, \
-                         hipGetErrorString(e_), __FILE__, __LINE__);                                           \
+// A call answers for its own errors: it reads none that other code has left with the runtime (so no hipGetLastError after a
+// launch), and takes back those that it reports, so that no later call finds them.
+int report(hipError_t e, const char *what, int line)
+{
+  (void)hipGetLastError();
+  return fail_no_ctx(e == hipErrorOutOfMemory ? MHLIK_ENOMEM : MHLIK_EHIP, "%s failed: %s (%s:%d)", what, hipGetErrorString(e), __FILE__, line);
+}
+#define PCHK(expr)                                                \
+  do {                                                            \
+    const hipError_t e_ = (expr);                                 \
+    if (e_ != hipSuccess) return report(e_, #expr, __LINE__);     \
   } while (0)
+
+template <typename V> struct Given {
+  typedef V type; // arguments convert to the kernel's parameters
+};
+template <typename... P>
+hipError_t launch(void (*kernel)(P...), dim3 grid, dim3 block, hipStream_t stream, typename Given<P>::type... args)
+{
+  void *at[] = {(void *)&args...};
+  return hipLaunchKernel((const void *)kernel, grid, block, at, 0, stream);
+}
 
 // The device a call names is current until the call returns; the caller's comes back.
 class OnDevice {
@@ -83,12 +98,11 @@ int quantize_launch(const T *x, int64_t rows, int64_t cols, int64_t rs, int64_t 
     const T *from = x + first * rs;
     uint8_t *d = data + first * blocks * kQ8Block, *s = scale + first * sstride;
     if (by_column)
-      hipLaunchKernelGGL(q8_columns_kernel<T>, dim3((unsigned)((n + kBlock - 1) / kBlock), (unsigned)blocks), dim3(kBlock), 0, stream, from,
-                         n, cols, cs, (uint32_t)blocks, (uint32_t)sstride, d, s);
+      PCHK(launch(q8_columns_kernel<T>, dim3((unsigned)((n + kBlock - 1) / kBlock), (unsigned)blocks), dim3(kBlock), stream, from, n, cols,
+                  cs, (uint32_t)blocks, (uint32_t)sstride, d, s));
     else
-      hipLaunchKernelGGL(q8_rows_kernel<T>, dim3((unsigned)((n * blocks * 16 + kBlock - 1) / kBlock)), dim3(kBlock), 0, stream,
-                         Q8Values{from, rs, cs, 0}, n * blocks, cols, (uint32_t)blocks, (uint32_t)sstride, d, s);
-    PCHK(hipGetLastError());
+      PCHK(launch(q8_rows_kernel<T>, dim3((unsigned)((n * blocks * 16 + kBlock - 1) / kBlock)), dim3(kBlock), stream,
+                  Q8Values{from, rs, cs, 0}, n * blocks, cols, (uint32_t)blocks, (uint32_t)sstride, d, s));
   }
   return MHLIK_OK;
 }
@@ -150,17 +164,17 @@ template <typename T> int product_part(const Q8Product &a, const Q8Values &value
     const int64_t groups = (groups16 + waves / ks - 1) / (waves / ks);
     const dim3 grid((unsigned)groups), block(waves * kWave);
     if (values.type && rf == 1)
-      hipLaunchKernelGGL((q8_skinny_kernel<T, 1, true>), grid, block, 0, stream, a, values, ks);
+      PCHK(launch((q8_skinny_kernel<T, 1, true>), grid, block, stream, a, values, ks));
     else if (values.type && rf == 2)
-      hipLaunchKernelGGL((q8_skinny_kernel<T, 2, true>), grid, block, 0, stream, a, values, ks);
+      PCHK(launch((q8_skinny_kernel<T, 2, true>), grid, block, stream, a, values, ks));
     else if (values.type)
-      hipLaunchKernelGGL((q8_skinny_kernel<T, 4, true>), grid, block, 0, stream, a, values, ks);
+      PCHK(launch((q8_skinny_kernel<T, 4, true>), grid, block, stream, a, values, ks));
     else if (rf == 1)
-      hipLaunchKernelGGL((q8_skinny_kernel<T, 1, false>), grid, block, 0, stream, a, values, ks);
+      PCHK(launch((q8_skinny_kernel<T, 1, false>), grid, block, stream, a, values, ks));
     else if (rf == 2)
-      hipLaunchKernelGGL((q8_skinny_kernel<T, 2, false>), grid, block, 0, stream, a, values, ks);
+      PCHK(launch((q8_skinny_kernel<T, 2, false>), grid, block, stream, a, values, ks));
     else
-      hipLaunchKernelGGL((q8_skinny_kernel<T, 4, false>), grid, block, 0, stream, a, values, ks);
+      PCHK(launch((q8_skinny_kernel<T, 4, false>), grid, block, stream, a, values, ks));
   } else if (a.blocks <= 2) {
     const int64_t high = kBlock / kWave * 16 * q8_thin_down(a.blocks, sizeof(T)), gm = (a.rows + high - 1) / high;
     const int64_t chunks = (a.draws + kQ8ThinDraws - 1) / kQ8ThinDraws;
@@ -174,13 +188,13 @@ template <typename T> int product_part(const Q8Product &a, const Q8Values &value
     const dim3 grid((unsigned)(gm * splits));
     const bool shifted = !aligned16(a.out) || a.os * (int64_t)sizeof(T) % 16 != 0; // rows that do not begin at 16 bytes
     if (a.blocks == 1 && !shifted)
-      hipLaunchKernelGGL((q8_thin_kernel<T, kWide, 1, false>), grid, dim3(kBlock), 0, stream, a, (int)splits, (int)each);
+      PCHK(launch((q8_thin_kernel<T, kWide, 1, false>), grid, dim3(kBlock), stream, a, (int)splits, (int)each));
     else if (a.blocks == 1)
-      hipLaunchKernelGGL((q8_thin_kernel<T, kWide, 1, true>), grid, dim3(kBlock), 0, stream, a, (int)splits, (int)each);
+      PCHK(launch((q8_thin_kernel<T, kWide, 1, true>), grid, dim3(kBlock), stream, a, (int)splits, (int)each));
     else if (!shifted)
-      hipLaunchKernelGGL((q8_thin_kernel<T, kWide, 2, false>), grid, dim3(kBlock), 0, stream, a, (int)splits, (int)each);
+      PCHK(launch((q8_thin_kernel<T, kWide, 2, false>), grid, dim3(kBlock), stream, a, (int)splits, (int)each));
     else
-      hipLaunchKernelGGL((q8_thin_kernel<T, kWide, 2, true>), grid, dim3(kBlock), 0, stream, a, (int)splits, (int)each);
+      PCHK(launch((q8_thin_kernel<T, kWide, 2, true>), grid, dim3(kBlock), stream, a, (int)splits, (int)each));
   } else {
     // Tiles of 256 do a quarter of the fetching per product that tiles of 64 would, and half of what tiles of 128 do; from
     // where they fill three quarters of the chip's 256 CUs they are the faster ones.
@@ -190,11 +204,10 @@ template <typename T> int product_part(const Q8Product &a, const Q8Values &value
       return fail_no_ctx(MHLIK_EINVAL, "too large a product (%lld x %lld)", (long long)a.rows, (long long)a.draws);
     const dim3 grid((unsigned)(tm * tn));
     if (side == 256)
-      hipLaunchKernelGGL((q8_tile_kernel<T, kWide, 256>), grid, dim3(kBlock), 0, stream, a, (int)tn, (int)(tm * tn));
+      PCHK(launch((q8_tile_kernel<T, kWide, 256>), grid, dim3(kBlock), stream, a, (int)tn, (int)(tm * tn)));
     else
-      hipLaunchKernelGGL((q8_tile_kernel<T, kWide, 128>), grid, dim3(kBlock), 0, stream, a, (int)tn, (int)(tm * tn));
+      PCHK(launch((q8_tile_kernel<T, kWide, 128>), grid, dim3(kBlock), stream, a, (int)tn, (int)(tm * tn)));
   }
-  PCHK(hipGetLastError());
   return MHLIK_OK;
 }
 
@@ -255,17 +268,18 @@ DrawPlan draw_plan(int64_t rows, int64_t n, void *workspace)
   return p;
 }
 
-template <typename T, int VEC, int VPT> void draw_long(const DrawArgs &a, const LongSpace &g, bool histo, bool collect, hipStream_t stream)
+template <typename T, int VEC, int VPT> int draw_long(const DrawArgs &a, const LongSpace &g, bool histo, bool collect, hipStream_t stream)
 {
   const dim3 grid((unsigned)(a.rows * g.groups));
-  hipLaunchKernelGGL((draw_top_kernel<T, VEC, VPT>), grid, dim3(kBlock), 0, stream, a, g, (int)histo);
+  PCHK(launch((draw_top_kernel<T, VEC, VPT>), grid, dim3(kBlock), stream, a, g, (int)histo));
   if (histo) { // a workgroup's histogram is added to the row's at the end: no more workgroups than fill the chip four times
     int groups = g.groups;
     while (groups > 1 && a.rows * groups > 1024) groups = (groups + 1) / 2;
-    hipLaunchKernelGGL((draw_histo_kernel<T, VEC, VPT>), dim3((unsigned)(a.rows * groups)), dim3(kBlock), 0, stream, a, g, groups);
+    PCHK(launch((draw_histo_kernel<T, VEC, VPT>), dim3((unsigned)(a.rows * groups)), dim3(kBlock), stream, a, g, groups));
   }
-  if (collect) hipLaunchKernelGGL((draw_collect_kernel<T, VEC, VPT>), grid, dim3(kBlock), 0, stream, a, g);
-  hipLaunchKernelGGL((draw_finish_kernel<T, VPT>), dim3((unsigned)a.rows), dim3(1024), 0, stream, a, g);
+  if (collect) PCHK(launch((draw_collect_kernel<T, VEC, VPT>), grid, dim3(kBlock), stream, a, g));
+  PCHK(launch((draw_finish_kernel<T, VPT>), dim3((unsigned)a.rows), dim3(1024), stream, a, g));
+  return MHLIK_OK;
 }
 
 template <typename T> int draw_part(const DrawArgs &a, const DrawPlan &p, hipStream_t stream)
@@ -278,31 +292,27 @@ template <typename T> int draw_part(const DrawArgs &a, const DrawPlan &p, hipStr
     const dim3 grid((unsigned)a.rows);
     const bool many = a.rows >= 512;
     if (many && a.n <= 128)
-      hipLaunchKernelGGL((draw_short_kernel<T, 64, 2>), grid, dim3(64), 0, stream, a, shift);
+      PCHK(launch((draw_short_kernel<T, 64, 2>), grid, dim3(64), stream, a, shift));
     else if (many && a.n <= 512)
-      hipLaunchKernelGGL((draw_short_kernel<T, 64, 8>), grid, dim3(64), 0, stream, a, shift);
+      PCHK(launch((draw_short_kernel<T, 64, 8>), grid, dim3(64), stream, a, shift));
     else if (a.n <= 512)
-      hipLaunchKernelGGL((draw_short_kernel<T, 256, 2>), grid, dim3(256), 0, stream, a, shift);
+      PCHK(launch((draw_short_kernel<T, 256, 2>), grid, dim3(256), stream, a, shift));
     else if (many && a.n <= 2048)
-      hipLaunchKernelGGL((draw_short_kernel<T, 256, 8>), grid, dim3(256), 0, stream, a, shift);
+      PCHK(launch((draw_short_kernel<T, 256, 8>), grid, dim3(256), stream, a, shift));
     else if (a.n <= 2048)
-      hipLaunchKernelGGL((draw_short_kernel<T, 512, 4>), grid, dim3(512), 0, stream, a, shift);
+      PCHK(launch((draw_short_kernel<T, 512, 4>), grid, dim3(512), stream, a, shift));
     else if (many)
-      hipLaunchKernelGGL((draw_short_kernel<T, 512, 16>), grid, dim3(512), 0, stream, a, shift);
+      PCHK(launch((draw_short_kernel<T, 512, 16>), grid, dim3(512), stream, a, shift));
     else
-      hipLaunchKernelGGL((draw_short_kernel<T, 1024, 8>), grid, dim3(1024), 0, stream, a, shift);
+      PCHK(launch((draw_short_kernel<T, 1024, 8>), grid, dim3(1024), stream, a, shift));
   } else if (!p.vpt) {
-    hipLaunchKernelGGL(draw_huge_kernel<T>, dim3((unsigned)a.rows), dim3(1024), 0, stream, a);
+    PCHK(launch(draw_huge_kernel<T>, dim3((unsigned)a.rows), dim3(1024), stream, a));
   } else {
     const bool histo = a.top_k || a.top_p || (a.top_k_all > 0 && a.top_k_all < a.n) || a.top_p_all < 1.0;
     const bool collect = histo || a.min_p || a.min_p_all > 0.0;
     constexpr int kVec = 16 / sizeof(T);
-    if (p.vpt == 16)
-      draw_long<T, kVec, 16>(a, p.space, histo, collect, stream);
-    else
-      draw_long<T, kVec, kLongVpt>(a, p.space, histo, collect, stream);
+    return p.vpt == 16 ? draw_long<T, kVec, 16>(a, p.space, histo, collect, stream) : draw_long<T, kVec, kLongVpt>(a, p.space, histo, collect, stream);
   }
-  PCHK(hipGetLastError());
   return MHLIK_OK;
 }
 

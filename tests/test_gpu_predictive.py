@@ -736,3 +736,33 @@ def test_forward_mode_is_refused(P):
         assert torch.equal(P.product(dual(x).detach(), w), plain[0])
         assert torch.equal(P.PosteriorPredictive(dual(x)).theta.scale, P.quantize(x).scale)  # keeps its draws detached
     assert torch.equal(P.product(x, w), plain[0]) and torch.equal(P.draw(z, u)[0], plain[1][0])
+
+
+def test_errors_of_other_calls_are_not_reported_again(P):
+    """A call on a device that is not there is refused, and the calls after it know nothing of it; nor of an error that
+    other code has left behind, which stays there for it."""
+    from mcmc_amd import Likelihood, _lib
+    from mcmc_amd.likelihood import synthetic_host
+
+    lib = _lib.load_mhlik()
+    x = torch.randn(100, 200, device="cuda")
+    z, u = torch.randn(3, 9000, device="cuda"), torch.rand(3, device="cuda")
+
+    def calls():
+        q = P.quantize(x)
+        return q.data.view(torch.uint8), P.product(x, q), P.product(q, q, torch.bfloat16), *P.draw(z, u, top_p=0.9), *P.draw(z[:, :50], u)
+
+    want = calls()
+    q = P.quantize(x)
+    nowhere = torch.cuda.device_count()
+    assert lib.mhlik_q8_quantize(x.data_ptr(), 2, 100, 200, 200, 1, q.data.data_ptr(), q.scale.data_ptr(), nowhere, None) == 3  # MHLIK_EHIP
+    assert "invalid device" in lib.mhlik_last_error(None).decode()
+    assert all(torch.equal(a, b) for a, b in zip(calls(), want))
+    assert lib.mhlik_q8_quantize(x.data_ptr(), 2, 100, 200, 200, 1, q.data.data_ptr(), q.scale.data_ptr(), nowhere, None) == 3
+    with Likelihood(3000, 5, device=0) as lk:  # the samplers' calls ask for the last error too
+        lk.upload(synthetic_host(3, 3000, 5))
+        assert math.isfinite(lk.loglik(np.zeros(5)))
+    assert lib.hipSetDevice(nowhere) != 0  # the runtime's own call
+    got = calls()
+    assert lib.hipGetLastError() != 0 and lib.hipGetLastError() == 0  # taken back before torch's kernels look for it
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
