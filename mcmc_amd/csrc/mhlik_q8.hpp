@@ -491,7 +491,10 @@ __global__ __launch_bounds__(kBlock, 2) void q8_thin_kernel(Q8Product a, int spl
 #if defined(__HIP_DEVICE_COMPILE__)
   constexpr int kDown = q8_thin_down(BLOCKS, (int)sizeof(T)), kN = kQ8ThinDraws; // draws at a time
   constexpr int kSide = kN * kQ8Block;
-  constexpr int kStores = kN / 64 * kDown * 2 * (int)sizeof(T) / 2; // a wave's, for one chunk of draws
+  // A wave's stores for one chunk of draws.  It writes 16 kDown rows of kN values, a store instruction takes 16 bytes a lane
+  // at most: there cannot be fewer, and more would only make the wait that counts them a longer one.
+  constexpr int kStores = 16 * kDown * kN * (int)sizeof(T) / (kWave * 16);
+  static_assert(kStores < 64, "what a wait can count to");
   __shared__ __align__(1024) uint8_t lds[2][BLOCKS * kSide];
   __shared__ __align__(1024) uint32_t lds_scale[2][kN];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x % kWave, r = lane & 15, g = lane >> 4;
@@ -593,6 +596,7 @@ __global__ __launch_bounds__(kBlock, 2) void q8_thin_kernel(Q8Product a, int spl
   for (int64_t j0 = from; j0 < to; j0 += kN, buf ^= 1, t += kSteps) {
     const bool more = j0 + kN < to;
     if (more) fetch(buf ^ 1, j0 + kN);
+    asm volatile("" ::: "memory"); // the fetch stays ahead of the chunk's stores
     if (t > 0 && j0 + kN <= to)
       chunk(buf, t, std::true_type{});
     else

@@ -766,3 +766,31 @@ def test_errors_of_other_calls_are_not_reported_again(P):
     got = calls()
     assert lib.hipGetLastError() != 0 and lib.hipGetLastError() == 0  # taken back before torch's kernels look for it
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("out", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("cols", [64, 200])
+@pytest.mark.parametrize("draws,stride", [(1000, 1000), (1001, 1001), (1024, 1024), (1024, 1031), (1023, 1040)])
+def test_product_narrow_with_several_chunks_a_workgroup(P, draws, stride, cols, out):
+    """Rows enough that a workgroup goes along four and more times 128 draws: two buffers in turn, lines carried from one
+    chunk to the next, rows of C that do and do not begin at 16 bytes.  Values as in the exact test, so that a stale one shows."""
+    from mcmc_amd import _lib
+
+    rows, dtype = 77_003, TYPES[out]
+    g = torch.Generator(device="cuda").manual_seed(draws + stride + cols)
+
+    def some(n):
+        v = (1 + torch.randint(0, 8, (n, cols), generator=g, device="cuda") / 8) * (torch.randint(0, 2, (n, cols), generator=g, device="cuda") * 2 - 1)
+        return v.double()
+
+    x, w = some(rows), some(draws)
+    xq, wq = P.quantize(x), P.quantize(w)
+    got = torch.full((rows + 1, stride), 77.0, dtype=dtype, device="cuda")
+    p = _lib.Q8Operands()
+    p.x, p.x_scale, p.w_data, p.w_scale = xq.data.data_ptr(), xq.scale.data_ptr(), wq.data.data_ptr(), wq.scale.data_ptr()
+    p.out, p.out_stride, p.rows, p.draws, p.cols = got.data_ptr(), stride, rows, draws, cols
+    p.out_type = {"f32": 2, "bf16": 3, "f16": 4}[out]
+    assert _lib.load_mhlik().mhlik_q8_product(C.byref(p), -1, torch.cuda.current_stream().cuda_stream) == 0
+    exact = torch.mm(x, w.t().contiguous()).to(dtype)  # at most 200 * 3.6: no infinities
+    assert torch.equal(got[:rows, :draws], exact)
+    assert (got[:rows, draws:] == 77).all() and (got[rows:] == 77).all()
