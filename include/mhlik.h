@@ -459,8 +459,11 @@ int mhlik_q8_quantize(const void *x, int32_t type, int64_t rows, int64_t cols, i
 
 /* out[i * out_stride + s] = sum_c x[i][c] w[s][c] over the values that the 8-bit rows stand for.  x may be 8-bit rows
  * (x_type MHLIK_T_Q8: x and x_scale) or values, which are quantized first, into the workspace.  out is float (products
- * and sums as exact as float sums are), bfloat16 or half (products as the 8-bit matrix instructions add them: 1.6e-5 of
- * the result's norm before the rounding).  The padding of 8-bit rows must be zeros, and out must not overlap the inputs.
+ * and sums as exact as float sums are), bfloat16 or half: from 65 rows on with products as the 8-bit matrix instructions
+ * add them, which keep about 16 bits below the largest of each 64 or 128: 1.6e-5 of the result's norm before the rounding,
+ * and more than that of a result that is small against its products; up to 64 rows as float has them, so that a row can
+ * differ in its last bit between a small batch and a large one.  The padding of 8-bit rows must be zeros, and out must not
+ * overlap the inputs.
  * 0 <= draws <= 2^29. */
 typedef struct mhlik_q8_operands {
   const void *x;          /* [rows] */

@@ -196,8 +196,10 @@ __global__ __launch_bounds__(kBlock) void q8_columns_kernel(const T *__restrict_
 //                        significant bits), products and sums are float's: 1.3e-7 of the result's norm at 8192 columns.
 //   narrow (16-bit C)    the scaled 8-bit matrix instruction, which takes the block's exponents as operands and runs at
 //                        twice the rate.  It aligns the products of one step before adding and keeps about 16 bits of
-//                        them: 1.6e-5 of the result's norm (measured, the same at 128 and 8192 columns), a
-//                        hundredth of what rounding C to bfloat16 costs and a tenth of float16's.
+//                        them: 1.5e-5 to 1.6e-5 of the result's norm with random signs, without a bias (measured, 64
+//                        to 8192 columns), 1e-6 with equal ones; a hundredth of what rounding C to bfloat16 costs and
+//                        a tenth of float16's, of whose values one in fifteen gets another last bit.  The few-rows
+//                        kernel is bound by reading the draws and multiplies the wide way whatever C's type.
 // All 128 columns of a step share their scales, so which column goes to which place of the instruction is free as long
 // as both operands agree.
 

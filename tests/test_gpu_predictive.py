@@ -794,3 +794,19 @@ def test_product_narrow_with_several_chunks_a_workgroup(P, draws, stride, cols, 
     exact = torch.mm(x, w.t().contiguous()).to(dtype)  # at most 200 * 3.6: no infinities
     assert torch.equal(got[:rows, :draws], exact)
     assert (got[:rows, draws:] == 77).all() and (got[rows:] == 77).all()
+
+
+@pytest.mark.parametrize("out", ["bf16", "f16"])
+@pytest.mark.parametrize("rows,draws,cols", [(2000, 1000, 64), (2000, 1000, 128), (2000, 1000, 256), (1000, 1000, 400), (1000, 1000, 4096), (4096, 4096, 1000)])
+def test_product_accuracy_of_16_bit_results(P, rows, draws, cols, out):
+    """What the 8-bit matrix instruction drops is 1.6e-5 of the result's norm, beside the rounding to 16 bits.  The two
+    errors are independent, so squares add up; twice the stated 1.6e-5, and 1 % of the rounding's share, which the same
+    values rounded after another error have within 1 / sqrt(2 rows draws) (1e-3 here)."""
+    g = torch.Generator(device="cuda").manual_seed(rows + cols)
+    x = P.quantize(torch.randn(rows, cols, generator=g, device="cuda"))
+    w = P.quantize(torch.randn(draws, cols, generator=g, device="cuda") / math.sqrt(cols))
+    exact = torch.mm(values(x), values(w).t().contiguous())
+    got = P.product(x, w, TYPES[out])
+    size = exact.norm()
+    off, rounding = ((got.double() - exact).norm() / size).item(), ((exact.to(TYPES[out]).double() - exact).norm() / size).item()
+    assert off ** 2 <= (1.01 * rounding) ** 2 + (2 * 1.6e-5) ** 2, (off, rounding)
