@@ -508,7 +508,8 @@ typedef struct mhlik_draw_rows {
   double temperature_all, top_p_all, min_p_all;
   int64_t *index;
   float *logp;
-  void *workspace;        /* mhlik_draw_workspace(rows, n) bytes at a multiple of 16 (may be 0) */
+  void *workspace;        /* mhlik_draw_workspace(rows, n) bytes at a multiple of 16: 0 up to 8192 columns, else
+                           * some 4 a weight, 0.75 GB at most */
   size_t workspace_bytes;
   int32_t top_k_all;
   int32_t z_type, u_type;

@@ -75,7 +75,7 @@ constexpr int64_t kMaxDraws = (int64_t)1 << 29;
 constexpr int64_t kPartRows = (int64_t)1 << 28;     // of a product or a quantization: 4 threads a row at most, or
 constexpr int64_t kPartBlocks = (int64_t)1 << 27;   // 16 a block
 constexpr int64_t kPartDrawRows = (int64_t)1 << 20; // of a draw: 1024 threads a row
-constexpr int64_t kPartWeights = (int64_t)1 << 27;  // of a draw's long rows, which bounds its workspace (1.1 GB)
+constexpr int64_t kPartWeights = (int64_t)1 << 27;  // of a draw's long rows, which bounds its workspace (0.75 GB)
 
 int check_rows8(const char *what, const void *data, const void *scale, int64_t rows)
 {

@@ -115,6 +115,19 @@ def test_workspace_sizes(lib):
     _refused(lib, lib.mhlik_draw_workspace(1, 0, C.byref(need)), "1 <= n")
 
 
+def test_the_draw_workspace_is_bounded(lib):
+    """Long rows go in parts: however many there are, their workspace stays below 0.75 GB.  It is largest for the shortest
+    ones, whose units are the least filled."""
+    need = C.c_size_t()
+    sizes = {}
+    for n in (8193, 8320, 10241, 20001, 65537, 131072, 1 << 20, 1 << 21):
+        for rows in (1, 100, 20000, (1 << 31) - 1):
+            assert lib.mhlik_draw_workspace(rows, n, C.byref(need)) == 0
+            sizes[n, rows] = need.value
+    assert max(sizes.values()) == sizes[8193, (1 << 31) - 1] < 750_000_000
+    assert lib.mhlik_draw_workspace((1 << 31) - 1, (1 << 21) + 1, C.byref(need)) == 0 and need.value == 0  # no units
+
+
 def test_struct_layouts_match_the_header():
     from mcmc_amd import _lib
 
