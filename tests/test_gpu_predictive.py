@@ -810,3 +810,24 @@ def test_product_accuracy_of_16_bit_results(P, rows, draws, cols, out):
     size = exact.norm()
     off, rounding = ((got.double() - exact).norm() / size).item(), ((exact.to(TYPES[out]).double() - exact).norm() / size).item()
     assert off ** 2 <= (1.01 * rounding) ** 2 + (2 * 1.6e-5) ** 2, (off, rounding)
+
+
+def test_posterior_predictive_in_a_graph(P):
+    """Captured as one, replayed with new rows, eager work between: one mean over a million draws, draws without a case."""
+    g = torch.Generator(device="cuda").manual_seed(12)
+    pp = P.PosteriorPredictive(torch.randn(1 << 20, 4, generator=g, device="cuda"))
+    x, u = torch.randn(2, 4, generator=g, device="cuda"), torch.rand(2, generator=g, device="cuda")
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        pp.probability(x), pp.case_deletion(x, u)
+    s.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = pp.probability(x), *pp.case_deletion(x, u, 0.9, top_p=0.95)
+    for _ in range(4):
+        x.copy_(torch.randn(2, 4, generator=g, device="cuda"))
+        u.copy_(torch.rand(2, generator=g, device="cuda"))
+        graph.replay()
+        torch.cuda.synchronize()
+        want = pp.probability(x), *pp.case_deletion(x, u, 0.9, top_p=0.95)
+        assert all(torch.equal(a, b) for a, b in zip(out, want))
