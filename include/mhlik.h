@@ -451,9 +451,11 @@ enum { MHLIK_T_Q8 = 0, MHLIK_T_F64 = 1, MHLIK_T_F32 = 2, MHLIK_T_BF16 = 3, MHLIK
  *   data [i][128 b + c] = e4m3(x 2^-k)   (to nearest even, from the exact quotient)
  *   scale[i][b]         = k + 127,       k the least integer in [-96, 119] with |x| <= 448 2^k for the block's finite x
  * data has 128 ceil(cols/128) bytes a row (columns past the last: 0), starts at a multiple of 16 bytes; scale has
- * 4 ceil(cols/512) bytes a row (spare ones: 127), starts at a multiple of 4.  Values that are not finite, or exceed 448 2^119, become NaN.
+ * 4 ceil(cols/512) bytes a row (spare ones: 127), starts at a multiple of 4.  Values that are not finite, or exceed
+ * 448 2^119, become NaN.
  * x[i * row_stride + c * col_stride], of any type but MHLIK_T_Q8; strides count elements and are not negative.
- * 0 <= rows <= 2^40, 1 <= cols <= 2^22.  Rows made elsewhere: scale bytes 31 .. 246, as these k have. */
+ * 0 <= rows <= 2^40, 1 <= cols <= 2^22.  Rows made elsewhere: scale bytes 31 .. 246, as these k have; no call looks at
+ * them first, and products of others come out differently by the type of out. */
 int mhlik_q8_quantize(const void *x, int32_t type, int64_t rows, int64_t cols, int64_t row_stride, int64_t col_stride,
                       uint8_t *data, uint8_t *scale, int32_t device, void *stream);
 
@@ -463,8 +465,7 @@ int mhlik_q8_quantize(const void *x, int32_t type, int64_t rows, int64_t cols, i
  * add them, which keep about 16 bits below the largest of each 64 or 128: 1.6e-5 of the result's norm before the rounding,
  * and more than that of a result that is small against its products; up to 64 rows as float has them, so that a row can
  * differ in its last bit between a small batch and a large one.  The padding of 8-bit rows must be zeros, and out must not
- * overlap the inputs.
- * 0 <= draws <= 2^29. */
+ * overlap the inputs.  0 <= draws <= 2^29. */
 typedef struct mhlik_q8_operands {
   const void *x;          /* [rows] */
   const uint8_t *x_scale; /* MHLIK_T_Q8 only */
@@ -485,16 +486,17 @@ int mhlik_q8_product(const mhlik_q8_operands *operands, int32_t device, void *st
 
 /* One column of each row of log weights z[i * stride + j], j < n (float, bfloat16 or half), by a random number u[i] in
  * [0, 1) (double or float):
- *   w_j = exp((z_j - max) / temperature);  z_j = -inf: 0
+ *   w_j = exp((z_j - max) / temperature);  z_j = -inf: 0;  +inf counts as the largest float
  *   in the order of z, largest first, equal ones by column, keep
  *     the first top_k                                              (top_k <= 0 or >= n: all)
  *     those before which less than top_p of the mass of these lies (top_p >= 1: all; the first always)
  *     those with w_j >= min(min_p, 1)                              (min_p <= 0: all)
  *   index[i] = the first column, in column order, at which the kept mass exceeds u of the whole of it
  *   logp[i]  = log(w_index / kept mass)                            (logp may be NULL)
- * Sums are taken in double; those that decide where top_p ends, in whole multiples of 2^-51 of the largest weight (of more
- * where the sum needs the bits: n 2^-51 of the mass off at most).  temperature 0: the largest, the lowest column of equal ones.  A row without a weight above
- * -inf, with a NaN, or whose u, temperature, top_p or min_p is NaN (or the temperature negative): index -1, logp NaN.
+ * Sums are taken in double; those that decide where top_p ends, in whole multiples of 2^-51 of the largest weight (of
+ * more where the sum needs the bits: n 2^-51 of the mass off at most).  temperature 0: the largest, the lowest column of
+ * equal ones; temperature_all is 0 or at least 1e-100.  A row without a weight above -inf, with a NaN, or whose u,
+ * temperature, top_p or min_p is NaN (or the temperature negative): index -1, logp NaN.
  * u outside [0, 1) counts as its nearest end.  temperature .. min_p: device arrays of one value a row, or NULL and the
  * *_all value for every row.  0 <= rows < 2^31, 1 <= n < 2^30. */
 typedef struct mhlik_draw_rows {

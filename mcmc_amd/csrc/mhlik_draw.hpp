@@ -749,7 +749,8 @@ template <typename T, int THREADS, int VPT> __global__ __launch_bounds__(THREADS
 //   finish   one workgroup a row: the border among the listed values, the unit in which the kept mass exceeds u of the
 //            whole, the column in it.  A row whose lists are too long goes the whole-row way.
 // Few rows are bound by the four kernels' latencies (one row of 131072, top-k and top-p: 3 + 4 + 6 + 9 us); many by double
-// instructions beside the reading (256 rows of 131072 without a choice: 35 us for `top`, 3.8 TB/s; with top-p 153 in all).
+// instructions beside the reading (256 rows of 131072 without a choice: 34 us for `top`, 3.9 TB/s; with top-p 142 in all).  What the
+// whole-row way takes is one workgroup's work: 64 rows of 50001 whose top-p ends in a crowded bin 142 us, others 37.
 
 constexpr int kLongBins = 512;
 constexpr int kLongList = 2048;  // listed values of a row

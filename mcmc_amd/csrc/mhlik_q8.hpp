@@ -628,8 +628,8 @@ __global__ __launch_bounds__(kBlock, 2) void q8_thin_kernel(Q8Product a, int spl
 // draws' fragment has draw 16 (a / 2) + 8 g + 4 (a % 2) + e as its row 8 a + 4 g + e, which leaves a lane with runs of
 // eight values of a row of C.
 // Rows past the end: the last one again, never stored.  Bound by the matrix instructions, of which a wave has one stream
-// and nothing beside it when it waits: 8192 x 8192 x 8192 to bfloat16 465 us, 2.36 PFLOP/s; 512 x 20000 x 4096 to float
-// 113 us, 1.21 PFLOP/s; tiles of 128, 2048 x 2048 x 2048 to bfloat16: 16 us, 1.06 PFLOP/s (of 256: 36 us).
+// and nothing beside it when it waits: 8192 x 8192 x 8192 to bfloat16 464 us, 2.37 PFLOP/s; 4096 x 4096 x 4096 to float
+// 115 us, 1.19 PFLOP/s; tiles of 128, 2048 x 2048 x 2048 to bfloat16: 16 us, 1.06 PFLOP/s (of 256: 36 us).
 __device__ __forceinline__ int q8_key(int row)
 {
   const int q = row >> 2;

@@ -69,7 +69,7 @@ _stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index:
 class Block8:
     """Rows of `cols` values in 8 bits: `data` float8_e4m3fn [rows, 128 ceil(cols / 128)], columns past the last 0, and
     `scale` uint8 [rows, 4 ceil(cols / 512)]: the 128 columns of block b stand for data * 2^(scale[:, b] - 127), with
-    scales from 31 to 246."""
+    scales from 31 to 246 (not checked, which would wait for the GPU; others give wrong products)."""
 
     __slots__ = ("data", "scale", "cols", "rows", "device")
 
@@ -177,7 +177,7 @@ def draw(z, u, temperature=1.0, top_k=None, top_p=None, min_p=None):
     """One column of each row of log weights z [rows, n] (float32, bfloat16, float16), by the random numbers u [rows] in
     [0, 1) (float64 or float32): (column int64 [rows], its log probability float32 [rows]).
 
-    Weights are exp((z - max) / temperature); of them the top_k largest are kept, of these the fewest that hold top_p of
+    Weights are exp((z - max) / temperature), +inf counting as the largest float; of them the top_k largest are kept, of these the fewest that hold top_p of
     their mass, of these the ones at least min_p times the largest; equal weights keep the lower columns.  The column is
     the first, in column order, at which the kept mass exceeds u of the whole.  temperature 0 takes the largest.  The
     four choices are numbers, or tensors of one value a row (float32; top_k int32); None is off, and so are top_k <= 0,
