@@ -486,7 +486,7 @@ int mhlik_q8_product(const mhlik_q8_operands *operands, int32_t device, void *st
 
 /* One column of each row of log weights z[i * stride + j], j < n (float, bfloat16 or half), by a random number u[i] in
  * [0, 1) (double or float):
- *   w_j = exp((z_j - max) / temperature);  z_j = -inf: 0;  +inf counts as the largest float
+ *   w_j = exp((z_j - max) / temperature);  0 below 2^-1020 and for -inf;  +inf counts as the largest float
  *   in the order of z, largest first, equal ones by column, keep
  *     the first top_k                                              (top_k <= 0 or >= n: all)
  *     those before which less than top_p of the mass of these lies (top_p >= 1: all; the first always)
