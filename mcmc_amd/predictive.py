@@ -177,11 +177,12 @@ def draw(z, u, temperature=1.0, top_k=None, top_p=None, min_p=None):
     """One column of each row of log weights z [rows, n] (float32, bfloat16, float16), by the random numbers u [rows] in
     [0, 1) (float64 or float32): (column int64 [rows], its log probability float32 [rows]).
 
-    Weights are exp((z - max) / temperature), +inf counting as the largest float; of them the top_k largest are kept, of these the fewest that hold top_p of
-    their mass, of these the ones at least min_p times the largest; equal weights keep the lower columns.  The column is
-    the first, in column order, at which the kept mass exceeds u of the whole.  temperature 0 takes the largest.  The
-    four choices are numbers, or tensors of one value a row (float32; top_k int32); None is off, and so are top_k <= 0,
-    top_p >= 1, min_p <= 0.  A row with nothing to draw (all -inf, or a NaN) gives column -1 and NaN."""
+    Weights are exp((z - max) / temperature), +inf counting as the largest float; of them the top_k largest are kept, of
+    these the fewest that hold top_p of their mass, of these the ones at least min_p times the largest; equal weights keep
+    the lower columns. The column is the first, in column order, at which the kept mass exceeds u of the whole.
+    temperature 0 takes the largest. The four choices are numbers, or tensors of one value a row (float32; top_k int32);
+    None is off, and so are top_k <= 0, top_p >= 1, min_p <= 0. A row with nothing to draw (all -inf, or a NaN) gives
+    column -1 and NaN."""
     device = _given("z", z, 2, _OUT)
     _same("u", _given("u", u, 1, _U), device)
     rows, n = z.shape
